@@ -32,6 +32,13 @@ from .ops import (
     silu_mul,
     tp_wait,
     workspace_bytes,
+    decode_attn_gqa_paged,
+    decode_attn_gqa_int8_paged,
+    paged_workspace_bytes,
+    rope_qkv_append_paged,
+    rope_axes,
+    evict_kvcache_paged,
+    evict_workspace_bytes,
 )
 
 __all__ = [
@@ -51,6 +58,13 @@ __all__ = [
     "silu_mul",
     "decode_attn_kvcache_tp",
     "tp_wait",
+    "decode_attn_gqa_paged",
+    "decode_attn_gqa_int8_paged",
+    "paged_workspace_bytes",
+    "rope_qkv_append_paged",
+    "rope_axes",
+    "evict_kvcache_paged",
+    "evict_workspace_bytes",
     "gqa_sk_fast",
     "qpt",
     "quant_int4_per_token",

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import pathlib
+import struct
 import threading
 
 LIB_PATH = pathlib.Path(__file__).resolve().with_name("libfqkv_b200.so")
@@ -38,6 +39,13 @@ class TpOut(ctypes.Structure):
     """fqkv_tp_out_t: where a tensor-parallel decode call sends its output."""
     _fields_ = [("world", ctypes.c_int32), ("rank", ctypes.c_int32), ("dst_offset", ctypes.c_int64),
                 ("dst", ctypes.c_void_p * TP_MAX_RANKS), ("counters", ctypes.c_void_p * TP_MAX_RANKS)]
+
+
+# fqkv_paged_kv_t, packed (no padding): format and a reserved word; page_size, num_pages, max_pages, B, Hkv, D;
+# the K, V, K-scale and V-scale pointers; K and V strides (page, head, token), K-scale and V-scale strides (page,
+# head); block table, its row stride, lengths.  One pack call, where filling a ctypes Structure field by field would
+# cost a decode step several microseconds.
+PAGED_KV = struct.Struct("=ii6q4Q6q4qQqQ")
 
 
 # name -> (restype, argtypes); the same set of symbols the header declares.
@@ -77,6 +85,12 @@ SIGNATURES = {
     "fqkv_argmax": (_INT, [ctypes.c_int32, _P, _I64, _I64, _P, _P, _P]),
     "fqkv_decode_attn_kvcache_out": (_INT, [ctypes.c_int32, ctypes.c_int32, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64,
                                             _I64, _I64, _I64, _P, _P, _SZ, _P]),
+    "fqkv_decode_attn_paged": (_INT, [_P, ctypes.c_int32, _P, _P, _I64, _P, _P, _SZ, _P]),
+    "fqkv_paged_workspace_bytes": (_SZ, [_INT, _I64, _I64, _I64, _I64, _I64, _INT]),
+    "fqkv_rope_append_paged": (_INT, [_P, ctypes.c_int32, _P, _I64, _P, _P, _I64, _P, _I64, ctypes.c_int32, _P, _P, _P,
+                                      _P, _I64, _I64, _P]),
+    "fqkv_evict_paged": (_INT, [_P, _P, _P, _P, _I64, _I64, _P, _SZ, _P]),
+    "fqkv_evict_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64]),
     "fqkv_decode_attn_kvcache_tp": (_INT, [ctypes.c_int32, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P,
                                            _P, _SZ, ctypes.POINTER(TpOut), _P]),
     "fqkv_tp_arrivals": (_I64, [ctypes.c_int32, _I64, _I64, _I64, _I64, _I64, _SZ]),

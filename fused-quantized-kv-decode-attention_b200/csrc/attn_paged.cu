@@ -1,0 +1,719 @@
+// Single-query attention over a paged KV cache with one length per sequence, sm_100a.
+//
+//   out[b, h] = sum_j softmax_j(q[b, h] . k[b, kh, j] / sqrt(D)) v[b, kh, j],   j < len[b], kh = h / G,
+// token j of sequence b in slot j % page of page table[b, j / page] of the pools [P, Hkv, page, D] (fp16,
+// or int8 codes with one fp16 scale per token and KV head).  An empty sequence gives zeros.  Optionally
+//   weights[b, kh, j] += sum over the group's heads of softmax_j.
+//
+// Bound: HBM (each K/V byte is read once for all query heads of its KV head; about one multiply-add per
+// byte and head).  Work split: the lengths are known only on the device, so the launch cannot cut the work
+// by sequence.  All key tiles of all (sequence, KV head) units stand in one line of T tiles and CTA c of a
+// persistent grid takes tiles [c * per, (c + 1) * per), per = ceil(T / grid): every CTA streams the same
+// number of bytes whatever the lengths are.  A unit that lies inside one CTA's range is finished there; one
+// that crosses a border leaves unnormalised fp32 parts (two slots per CTA: the unit its range begins in and
+// the one it ends in), merged by the next launch in tile order, so results do not depend on timing.
+//
+//  * Warp 4 is the producer.  A tile is fetched as boxes of 16, 32, 64 or 128 keys (the largest that divides
+//    the page), each inside one page, by 4-D tensor copies over (D, token, head, page) with any 16-byte
+//    strides -- tokens outside heads or inside.  The lanes of the warp issue one box each.  Page numbers are
+//    read 32 boxes ahead.
+//  * Warps 0-3 take 16 (or 32) keys of a tile each.  S = Q K^T by mma m16n8k16 with the heads as rows;
+//    O^T += V^T P^T with the head dimension as rows, where the probabilities are the B operand exactly as
+//    the score accumulators hold them and 8 heads fill all 8 columns: half the MMAs and half the accumulator
+//    registers of the P V order, which leaves half of its 16 rows empty.  More than 8 heads take two column
+//    tiles, so up to 16 heads share one pass over K and V.
+//  * int8: a code becomes the exact fp16 number by one byte permute into 1024 + (code + 128) and one
+//    subtraction.  The K scale multiplies the score.  The V scale multiplies the probability before it is
+//    rounded to fp16, times a power of two that puts the unit's largest V scale so far in [2^13, 2^14): small
+//    scales keep all their bits, and the factor leaves exactly at the end of the unit.
+//  * Scores, maxima, sums and outputs are fp32; the probabilities are rounded to fp16 once, as the operand of
+//    the second product (half an ulp is 2^-12 relative, random over the keys); the output is rounded once.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+#include <type_traits>
+
+#include "device_common.cuh"
+#include "kernels.h"
+
+namespace fqkv {
+namespace {
+
+constexpr int kWarps = 4;          // consumer warps
+constexpr int kThr = 32 * (kWarps + 1);
+constexpr int kMergeHeads = 4;     // heads merged per epilogue pass
+
+template <int D, bool kI8>
+struct Cfg {
+  static constexpr int KPW = (kI8 && D == 64) ? 32 : 16;  // keys of a tile per consumer warp
+  static constexpr int TK = kWarps * KPW;                 // keys per tile
+  static constexpr int kBlocks = kI8 ? 1 : D / 64;        // column blocks of a tile (128-byte fp16 rows)
+  static constexpr int RB = kI8 ? D : 128;                // bytes of a row of a column block
+  static constexpr int kBlockBytes = TK * RB;
+  static constexpr int kTileBytes = kBlocks * kBlockBytes;  // K (or V) of one tile
+  static constexpr int kScaleBytes = kI8 ? 2 * TK : 0;
+  static constexpr int kStageBytes = 2 * kTileBytes + (kI8 ? 1024 : 0);  // scales in a 1 KB tail: tiles stay aligned
+  static constexpr int kCtas = D == 128 ? (kI8 ? 3 : 2) : (kI8 ? 3 : 4);
+  static constexpr int kStages = 3;
+  static constexpr size_t kRingBytes = size_t(kStages) * kStageBytes;
+  static constexpr size_t kBarBytes = 2 * kStages * sizeof(uint64_t);
+  static constexpr int kHeadStride = D + 4;               // floats; makes the epilogue's stores conflict-free
+  static constexpr size_t kMergeBytes = size_t(kWarps) * (2 * kPagedMaxHeads + kMergeHeads * kHeadStride) * sizeof(float);
+  static constexpr size_t kSmemBytes = 1024 + kRingBytes + kBarBytes + kMergeBytes;
+};
+
+// Tiled tensor copy of one box of one page into this CTA's shared memory.
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w),
+        "r"(smem_u32(bar))
+      : "memory");
+}
+
+// Byte offset of 16-byte chunk `c` of row `row` in a column block written with the swizzle of its row width.
+template <int RB>
+__device__ __forceinline__ uint32_t blk_off(int row, int c) {
+  if constexpr (RB == 128) return uint32_t(row * 128 + ((c ^ (row & 7)) << 4));
+  else return uint32_t(row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
+}
+template <int D, bool kI8>
+__device__ __forceinline__ uint32_t tile_off(int row, int chunk) {
+  if constexpr (kI8) return blk_off<Cfg<D, kI8>::RB>(row, chunk);
+  else return uint32_t((chunk >> 3) * Cfg<D, kI8>::kBlockBytes) + blk_off<128>(row, chunk & 7);
+}
+
+// ------------------------------------------------------------------ the line of tiles
+// One stretch of tiles of one unit inside a CTA's range.
+struct Part {
+  int b, kh, grp;  // the unit: sequence, KV head, head group
+  int len, nt;     // the sequence's tokens and tiles
+  int t0, t1;      // tiles [t0, t1)
+};
+
+// The walk over a CTA's range; every warp runs its own, all lanes alike.
+struct Walk {
+  const int* lens;
+  int B, cap, tk, units_per_seq, groups;
+  int per, cur, end;  // tiles per CTA; the range's position and end in the line
+  int b, u, t, len, nt;
+
+  __device__ __forceinline__ int length(int i) const { return max(0, min(cap, lens[i])); }
+  __device__ __forceinline__ int tiles(int n) const { return (n + tk - 1) / tk; }
+
+  __device__ __forceinline__ void init(const PagedLaunch& a, int tile_keys) {
+    const int lane = threadIdx.x & 31;
+    lens = a.seq_lens;
+    B = a.B;
+    cap = a.cap;
+    tk = tile_keys;
+    groups = a.groups;
+    units_per_seq = a.Hkv * a.groups;
+    int sum = 0;
+    for (int i = lane; i < B; i += 32) sum += tiles(length(i));
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    const int total = sum * units_per_seq;
+    const int grid = int(gridDim.x);
+    per = max(1, (total + grid - 1) / grid);
+    cur = int(min(int64_t(total), int64_t(blockIdx.x) * per));
+    end = min(total, cur + per);
+    b = u = t = len = nt = 0;
+    if (cur >= end) return;
+    int base = 0;
+    for (int i0 = 0; i0 < B; i0 += 32) {
+      const int n = i0 + lane < B ? length(i0 + lane) : 0;
+      int incl = tiles(n) * units_per_seq;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += v;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, base + incl > cur);
+      if (past) {
+        const int l = __ffs(int(past)) - 1;
+        b = i0 + l;
+        len = __shfl_sync(0xffffffffu, n, l);
+        nt = tiles(len);
+        const int r = cur - (base + __shfl_sync(0xffffffffu, incl, l) - nt * units_per_seq);
+        u = r / nt;
+        t = r - u * nt;
+        return;
+      }
+      base += __shfl_sync(0xffffffffu, incl, 31);
+    }
+  }
+
+  __device__ __forceinline__ bool next(Part& p) {
+    if (cur >= end) return false;
+    if (t >= nt) {  // past the unit: the next one, of the next sequence that has tokens
+      t = 0;
+      if (++u >= units_per_seq) {
+        u = 0;
+        do {
+          if (++b >= B) {  // only if the lengths changed meanwhile
+            cur = end;
+            return false;
+          }
+          len = length(b);
+          nt = tiles(len);
+        } while (nt == 0);
+      }
+    }
+    p.b = b;
+    p.kh = u / groups;
+    p.grp = u - p.kh * groups;
+    p.len = len;
+    p.nt = nt;
+    p.t0 = t;
+    p.t1 = min(nt, t + (end - cur));
+    cur += p.t1 - t;
+    t = p.t1;
+    return true;
+  }
+};
+
+__device__ __forceinline__ void store_out(const PagedLaunch& a, size_t idx, float v) {
+  if (a.out_bf16) static_cast<__nv_bfloat16*>(a.out)[idx] = __float2bfloat16_rn(v);
+  else static_cast<__half*>(a.out)[idx] = __float2half_rn(v);
+}
+
+// Two halves 1024 + u, 1024 + v of two bytes u, v of x (code + 128) minus 1152: the codes, exactly.
+template <uint32_t kSel>
+__device__ __forceinline__ uint32_t codes_to_half2(uint32_t x) {
+  uint32_t h;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(h) : "r"(x), "r"(0x64646464u), "n"(kSel));
+  const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&h), __half2half2(__ushort_as_half(0x6480u)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// kNT: column tiles of 8 heads (1: up to 8 heads per unit, 2: up to 16).
+template <int D, bool kI8, int kNT>
+__global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(const __grid_constant__ PagedLaunch a) {
+  using C = Cfg<D, kI8>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((uint32_t(1024) - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kRingBytes);
+  uint64_t* empty = full + C::kStages;
+  float* sm_m = reinterpret_cast<float*>(empty + C::kStages);  // [warps][kPagedMaxHeads]
+  float* sm_l = sm_m + kWarps * kPagedMaxHeads;
+  float* sm_o = sm_l + kWarps * kPagedMaxHeads;                // [warps][kMergeHeads][kHeadStride]
+  __shared__ int abort_flag;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const WaitCtl wc{a.status, a.timeout_ns};
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], kWarps);
+    }
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == kWarps && lane == 0) {
+    prefetch_tensormap(&a.tmK);
+    prefetch_tensormap(&a.tmV);
+  }
+  __syncthreads();
+  pdl_launch_dependents();
+  pdl_wait_primary();
+
+  Walk walk;
+  walk.init(a, C::TK);
+  Part p;
+
+  // ------------------------------------------------------------ producer
+  if (warp == kWarps) {
+    if (!a.debug_skip_loads) {
+      const int br = a.box;             // keys per box
+      const int nb = C::TK / br;        // boxes per tile: 1, 2, 4 or 8
+      constexpr int kKinds = kI8 ? 4 : 2 * C::kBlocks;  // copies per box
+      const int job_box = lane / kKinds, kind = lane % kKinds;
+      int it = 0;
+      bool ok = true;
+      while (ok && walk.next(p)) {
+        const int* row = a.table + int64_t(p.b) * a.table_stride;
+        const int first = p.t0 * nb;                                   // boxes counted from the sequence's start
+        const int last = min(p.t1 * nb, (p.len + br - 1) / br);        // boxes that hold tokens
+        auto page_of = [&](int box) { return box < last ? row[(int64_t(box) * br) / a.page] : 0; };
+        int ids = page_of(first + lane), ids_next = page_of(first + 32 + lane), at = 0;
+        for (int t = p.t0; t < p.t1 && ok; ++t, ++it, at += nb) {
+          if (at == 32) {  // nb divides 32
+            ids = ids_next;
+            ids_next = page_of(t * nb + 32 + lane);
+            at = 0;
+          }
+          const int st = it % C::kStages;
+          if (it >= C::kStages) {
+            const bool free_stage = !*reinterpret_cast<volatile int*>(&abort_flag) &&
+                                    mbar_wait(&empty[st], ((it / C::kStages) - 1) & 1, wc, kDevTimeoutEmpty);
+            if (!__all_sync(0xffffffffu, free_stage)) {
+              ok = false;
+              break;
+            }
+          }
+          const int boxes = min(nb, last - t * nb);  // a box past the last token is not fetched
+          if (lane == 0)
+            mbar_arrive_expect_tx(&full[st], uint32_t(boxes) * br * uint32_t(2 * C::kBlocks * C::RB + (kI8 ? 4 : 0)));
+          __syncwarp();
+          int id = __shfl_sync(0xffffffffu, ids, (at + job_box) & 31);
+          if (job_box < boxes) {
+            const int tok = int((int64_t(t) * C::TK + job_box * br) % a.page);
+            const bool known = unsigned(id) < unsigned(a.num_pages);
+            if (!known && kind == 0) atomicCAS(a.status, kDevOk, kDevBadPage);
+            uint8_t* stage = smem + size_t(st) * C::kStageBytes;
+            if (kI8 && kind >= 2) {
+              // a number outside the pool: some scales, for the zero codes of its keys
+              const int pg = known ? id : 0;
+              const __half* src = kind == 2 ? a.Ks + int64_t(pg) * a.ks_page + int64_t(p.kh) * a.ks_head + tok
+                                            : a.Vs + int64_t(pg) * a.vs_page + int64_t(p.kh) * a.vs_head + tok;
+              bulk_g2s(stage + 2 * C::kTileBytes + (kind - 2) * C::kScaleBytes + job_box * br * 2, src, uint32_t(br) * 2,
+                       &full[st]);
+            } else {
+              const bool is_v = kI8 ? kind == 1 : kind >= C::kBlocks;
+              const int blk = kI8 ? 0 : kind % C::kBlocks;
+              uint8_t* dst = stage + (is_v ? C::kTileBytes : 0) + blk * C::kBlockBytes + job_box * br * C::RB;
+              // outside the pool the copy unit writes zeros and reads nothing
+              tma_load_4d(dst, is_v ? &a.tmV : &a.tmK, blk * 64, tok, p.kh, known ? id : a.num_pages, &full[st]);
+            }
+          }
+        }
+      }
+      if (!ok && lane == 0) {
+        // The consumers gave up: wait (bounded) for the copies in flight before the CTA's memory goes.
+        for (int j = (it > C::kStages ? it - C::kStages : 0); j < it; ++j)
+          mbar_wait(&full[j % C::kStages], (j / C::kStages) & 1, wc, kDevTimeoutDrain);
+      }
+    }
+    return;
+  }
+
+  // ------------------------------------------------------------ consumers
+  const int g = lane >> 2;   // mma row of S: head g (and g + 8)
+  const int t4 = lane & 3;
+  const int mi = lane >> 3;  // ldmatrix matrix of this lane
+  const int rr = lane & 7;   // and row in it
+  const uint32_t ring = smem_u32(smem);
+  const int ct = threadIdx.x;
+  bool alive = true;
+  int it = 0;
+
+  // sequences without tokens: zeros
+  for (int b = int(blockIdx.x); b < a.B; b += int(gridDim.x))
+    if (a.seq_lens[b] <= 0)
+      for (int i = ct; i < a.Hq * D; i += 32 * kWarps) store_out(a, size_t(b) * a.Hq * D + i, 0.f);
+
+  int4 info = make_int4(0, 0, 0, 0);
+  while (walk.next(p)) {
+    const int h0 = p.kh * a.G + p.grp * a.GP;
+    const int gvalid = min(a.GP, a.G - p.grp * a.GP);
+    const size_t row_base = size_t(p.b) * a.Hq + h0;
+
+    // Q fragments.  fp16: k = 2t, 2t + 1 and 2t + 8, 2t + 9 of each 16 dimensions; int8: the four
+    // consecutive dimensions 4t .. 4t + 3 in their place, as the lane finds them in a row of codes.
+    uint32_t qa[D / 16][2 * kNT];
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+      const bool on = g + 8 * nt < gvalid;
+      const __half* qrow = static_cast<const __half*>(a.q) + (row_base + g + 8 * nt) * D;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint2 v = make_uint2(0u, 0u);
+        if (on) {
+          const int o0 = 16 * kk + (kI8 ? 4 * t4 : 2 * t4);
+          v.x = *reinterpret_cast<const uint32_t*>(qrow + o0);
+          v.y = *reinterpret_cast<const uint32_t*>(qrow + o0 + (kI8 ? 2 : 8));
+        }
+        qa[kk][2 * nt] = v.x;
+        qa[kk][2 * nt + 1] = v.y;
+      }
+    }
+    float o[kNT][D / 16][4];
+    float m_run[kNT], l_run[kNT];
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+      m_run[nt] = -INFINITY;
+      l_run[nt] = 0.f;
+#pragma unroll
+      for (int dd = 0; dd < D / 16; ++dd) o[nt][dd][0] = o[nt][dd][1] = o[nt][dd][2] = o[nt][dd][3] = 0.f;
+    }
+    float frame = 0.f;  // int8: the power of two in the probabilities (0: none yet)
+
+    for (int t = p.t0; t < p.t1; ++t, ++it) {
+      const int st = it % C::kStages;
+      if (alive) {
+        const bool ok = mbar_wait(&full[st], (it / C::kStages) & 1, wc, kDevTimeoutFull) &&
+                        !*reinterpret_cast<volatile int*>(&abort_flag);
+        alive = __all_sync(0xffffffffu, ok);
+        if (!alive && lane == 0) abort_flag = 1;
+      }
+      if (!alive) continue;
+      const uint32_t sk = ring + uint32_t(st) * C::kStageBytes;
+      const uint32_t sv = sk + C::kTileBytes;
+      const __half* scales = reinterpret_cast<const __half*>(smem + size_t(st) * C::kStageBytes + 2 * C::kTileBytes);
+      const int k0 = t * C::TK;
+
+      auto tile = [&](auto mask_tag) {
+        constexpr bool kMask = decltype(mask_tag)::value;
+        constexpr int NJ = C::KPW / 8;
+        const int r0 = warp * C::KPW;
+        // ---- S = Q K^T
+        float sc[NJ][4];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+        auto mma_s = [&](float(&d)[4], int kk, uint32_t b0, uint32_t b1) {
+          if constexpr (kNT == 1) mma_16816(d, qa[kk][0], 0u, qa[kk][1], 0u, b0, b1);
+          else mma_16816(d, qa[kk][0], qa[kk][2], qa[kk][1], qa[kk][3], b0, b1);
+        };
+#pragma unroll
+        for (int kb = 0; kb < C::KPW / 16; ++kb) {
+          const int row = r0 + 16 * kb + ((mi >> 1) << 3) + rr;
+          if constexpr (!kI8) {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              uint32_t b0, b1, b2, b3;
+              ldmatrix_x4(sk + tile_off<D, kI8>(row, 2 * kk + (mi & 1)), b0, b1, b2, b3);
+              mma_s(sc[2 * kb], kk, b0, b1);
+              mma_s(sc[2 * kb + 1], kk, b2, b3);
+            }
+          } else {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; kk += 2) {
+              uint32_t b[4];  // (keys 0-7, chunk kk), (keys 0-7, kk + 1), (keys 8-15, kk), (keys 8-15, kk + 1)
+              ldmatrix_x4(sk + tile_off<D, kI8>(row, kk + (mi & 1)), b[0], b[1], b[2], b[3]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t x = b[i] ^ 0x80808080u;
+                mma_s(sc[2 * kb + (i >> 1)], kk + (i & 1), codes_to_half2<0x4140>(x), codes_to_half2<0x4342>(x));
+              }
+            }
+          }
+        }
+        // ---- online softmax in the log2 domain; this lane: heads g (+ 8), keys k0 + r0 + 8j + 2 t4 + e
+        float vs[NJ][2];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const int kq = r0 + 8 * j + 2 * t4;
+          float ks0 = a.sm_scale_log2, ks1 = a.sm_scale_log2;
+          if constexpr (kI8) {
+            const float2 kf = __half22float2(*reinterpret_cast<const __half2*>(scales + kq));
+            const float2 vf = __half22float2(*reinterpret_cast<const __half2*>(scales + C::TK + kq));
+            ks0 *= kf.x;
+            ks1 *= kf.y;
+            vs[j][0] = (!kMask || k0 + kq < p.len) ? vf.x : 0.f;
+            vs[j][1] = (!kMask || k0 + kq + 1 < p.len) ? vf.y : 0.f;
+          }
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt) {
+            sc[j][2 * nt] = (!kMask || k0 + kq < p.len) ? sc[j][2 * nt] * ks0 : -INFINITY;
+            sc[j][2 * nt + 1] = (!kMask || k0 + kq + 1 < p.len) ? sc[j][2 * nt + 1] * ks1 : -INFINITY;
+          }
+          if (a.scores) {
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt)
+              if (g + 8 * nt < gvalid && (!kMask || k0 + kq < p.len))  // cap is even: the pair stays in the row
+                *reinterpret_cast<float2*>(a.scores + (row_base + g + 8 * nt) * size_t(a.cap) + k0 + kq) =
+                    make_float2(sc[j][2 * nt], sc[j][2 * nt + 1]);
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) mx = fmaxf(mx, fmaxf(sc[j][2 * nt], sc[j][2 * nt + 1]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const float m_new = fmaxf(m_run[nt], mx);
+          if (__any_sync(0xffffffffu, m_new > m_run[nt])) {
+            const float alpha = (m_new == -INFINITY) ? 1.f : ex2(m_run[nt] - m_new);
+            // O^T's columns are heads 2 t4 and 2 t4 + 1
+            const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t4);
+            const float a1 = __shfl_sync(0xffffffffu, alpha, 8 * t4 + 4);
+#pragma unroll
+            for (int dd = 0; dd < D / 16; ++dd) {
+              o[nt][dd][0] *= a0;
+              o[nt][dd][1] *= a1;
+              o[nt][dd][2] *= a0;
+              o[nt][dd][3] *= a1;
+            }
+            l_run[nt] *= alpha;
+            m_run[nt] = m_new;
+          }
+          const float mu = (m_run[nt] == -INFINITY) ? 0.f : m_run[nt];
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) {
+            sc[j][2 * nt] = ex2(sc[j][2 * nt] - mu);
+            sc[j][2 * nt + 1] = ex2(sc[j][2 * nt + 1] - mu);
+            l_run[nt] += sc[j][2 * nt] + sc[j][2 * nt + 1];
+          }
+        }
+        if constexpr (kI8) {
+          float vmax = 0.f;
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) vmax = fmaxf(vmax, fmaxf(vs[j][0], vs[j][1]));
+          vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 1));
+          vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));  // the same in every lane
+          if (vmax * frame >= 16384.f || (frame == 0.f && vmax > 0.f)) {
+            float k;
+            const float f = frame_for(vmax, k);
+            const float r = frame == 0.f ? 0.f : f / frame;  // powers of two; O is 0 before the first frame
+            frame = f;
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+              for (int dd = 0; dd < D / 16; ++dd)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[nt][dd][e] *= r;
+          }
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) {
+            vs[j][0] *= frame;
+            vs[j][1] *= frame;
+          }
+        }
+        // ---- O^T += V^T P^T
+#pragma unroll
+        for (int kb = 0; kb < C::KPW / 16; ++kb) {
+          uint32_t pb[kNT][2];
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float* s2 = &sc[2 * kb + i][2 * nt];
+              pb[nt][i] = kI8 ? pack_half2(s2[0] * vs[2 * kb + i][0], s2[1] * vs[2 * kb + i][1]) : pack_half2(s2[0], s2[1]);
+            }
+          const int row = r0 + 16 * kb + ((mi & 1) << 3) + rr;
+          if constexpr (!kI8) {
+            // The slots past the last token may hold anything, and 0 * inf is NaN: they are masked to zero.
+            uint32_t vm0 = 0xffffffffu, vm1 = 0xffffffffu;
+            if constexpr (kMask) {
+              const int kq = k0 + r0 + 16 * kb + 2 * t4;
+              vm0 = (kq < p.len ? 0x0000ffffu : 0u) | (kq + 1 < p.len ? 0xffff0000u : 0u);
+              vm1 = (kq + 8 < p.len ? 0x0000ffffu : 0u) | (kq + 9 < p.len ? 0xffff0000u : 0u);
+            }
+#pragma unroll
+            for (int dd = 0; dd < D / 16; ++dd) {
+              uint32_t v0, v1, v2, v3;  // (keys 0-7, dims 0-7), (keys 8-15, dims 0-7), (0-7, 8-15), (8-15, 8-15)
+              ldmatrix_x4_trans(sv + tile_off<D, kI8>(row, 2 * dd + (mi >> 1)), v0, v1, v2, v3);
+              if constexpr (kMask) {
+                v0 &= vm0;
+                v1 &= vm1;
+                v2 &= vm0;
+                v3 &= vm1;
+              }
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt) mma_16816(o[nt][dd], v0, v2, v1, v3, pb[nt][0], pb[nt][1]);
+            }
+          } else {
+            // a transposed 8 x 16-byte matrix: keys 2 t4, 2 t4 + 1 of dimensions 2g, 2g + 1; row g of the MMA
+            // is dimension 2g, row g + 8 is 2g + 1
+#pragma unroll
+            for (int dd = 0; dd < D / 16; dd += 2) {
+              uint32_t v[4];  // (keys 0-7, chunk dd), (keys 8-15, dd), (0-7, dd + 1), (8-15, dd + 1)
+              ldmatrix_x4_trans(sv + tile_off<D, kI8>(row, dd + (mi >> 1)), v[0], v[1], v[2], v[3]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) v[i] ^= 0x80808080u;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t lo0 = codes_to_half2<0x4240>(v[2 * i]), hi0 = codes_to_half2<0x4341>(v[2 * i]);
+                const uint32_t lo1 = codes_to_half2<0x4240>(v[2 * i + 1]), hi1 = codes_to_half2<0x4341>(v[2 * i + 1]);
+#pragma unroll
+                for (int nt = 0; nt < kNT; ++nt) mma_16816(o[nt][dd + i], lo0, hi0, lo1, hi1, pb[nt][0], pb[nt][1]);
+              }
+            }
+          }
+        }
+      };
+      if (k0 + C::TK <= p.len) tile(std::false_type{});
+      else tile(std::true_type{});
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+
+    // ---- end of the part: merge the warps; write the output (a whole unit) or one part of it
+    const bool whole = p.t0 == 0 && p.t1 == p.nt;
+    const size_t slot = size_t(blockIdx.x) * 2 + (p.t0 == 0 ? 1 : 0);
+    const float unframe = (kI8 && frame != 0.f) ? 1.f / frame : 1.f;
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+      float l = l_run[nt];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if (t4 == 0) {
+        sm_m[warp * kPagedMaxHeads + g + 8 * nt] = m_run[nt];
+        sm_l[warp * kPagedMaxHeads + g + 8 * nt] = l;
+      }
+    }
+    for (int hp = 0; hp < gvalid; hp += kMergeHeads) {
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int hl = 8 * nt + 2 * t4 + e - hp;
+          if (hl >= 0 && hl < kMergeHeads) {
+            float* dst = sm_o + (warp * kMergeHeads + hl) * C::kHeadStride + (kI8 ? 2 * g : g);
+#pragma unroll
+            for (int dd = 0; dd < D / 16; ++dd) {
+              dst[16 * dd] = o[nt][dd][e] * unframe;
+              dst[16 * dd + (kI8 ? 1 : 8)] = o[nt][dd][2 + e] * unframe;
+            }
+          }
+        }
+      }
+      named_bar_sync(1, 32 * kWarps);
+      const int nh = min(kMergeHeads, gvalid - hp);
+      for (int idx = ct; idx < nh * D; idx += 32 * kWarps) {
+        const int hl = idx / D, d = idx - hl * D;
+        const int hh = hp + hl;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w * kPagedMaxHeads + hh]);
+        float L = 0.f, O = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float mw = sm_m[w * kPagedMaxHeads + hh];
+          // a warp whose keys all lie past the last token has no say (its sums are 0; a NaN there stays a NaN)
+          const float wt = (mw == -INFINITY) ? (M == -INFINITY ? 1.f : 0.f) : ex2(mw - M);
+          L += wt * sm_l[w * kPagedMaxHeads + hh];
+          O += wt * sm_o[(w * kMergeHeads + hl) * C::kHeadStride + d];
+        }
+        if (whole) {
+          store_out(a, (row_base + hh) * D + d, O / L);
+          if (d == 0 && a.scores) a.row_ml[row_base + hh] = make_float2(M, L);
+        } else {
+          if (d == 0) a.part_ml[slot * a.GP + hh] = make_float2(M, L);
+          a.part_o[(slot * a.GP + hh) * D + d] = O;
+        }
+      }
+      named_bar_sync(1, 32 * kWarps);
+    }
+    if (p.t0 == 0 && p.t1 < p.nt)  // this CTA holds the unit's first part; the merge starts here
+      info = make_int4(int(row_base), gvalid, 1 + (p.nt - p.t1 + walk.per - 1) / walk.per, 0);
+  }
+  if (ct == 0 && a.part_info) a.part_info[blockIdx.x] = info;
+}
+
+// ------------------------------------------------------------------ merge of the units that cross a border
+// CTA c: the unit whose first part is CTA c's (part_info[c]); its parts are slot 1 of CTA c and slot 0 of the
+// following ones, merged in that order.  blockIdx.y: a head.  Thread: one dimension of one group of parts.
+constexpr int kCombineThreads = 256;
+
+__global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const __grid_constant__ PagedLaunch a) {
+  pdl_launch_dependents();
+  pdl_wait_primary();
+  __shared__ float sm_o[kCombineThreads], sm_m[kCombineThreads / 64], sm_l[kCombineThreads / 64];
+  const int4 info = a.part_info[blockIdx.x];  // row of the unit's first head, heads, parts
+  const int h = int(blockIdx.y);
+  if (h >= info.y) return;
+  const int D = a.D, groups = kCombineThreads / D;
+  const int gi = threadIdx.x / D, d = threadIdx.x - gi * D;
+  float M = -INFINITY, L = 0.f, O = 0.f;
+#pragma unroll 8
+  for (int s = gi; s < info.z; s += groups) {
+    const size_t slot = (size_t(blockIdx.x) + s) * 2 + (s == 0 ? 1 : 0);
+    const float2 ml = a.part_ml[slot * a.GP + h];
+    const float os = a.part_o[(slot * a.GP + h) * D + d];
+    const float Mn = fmaxf(M, ml.x);
+    const float wa = (Mn == -INFINITY) ? 1.f : ex2(M - Mn);
+    const float wb = (Mn == -INFINITY) ? 1.f : ex2(ml.x - Mn);
+    L = L * wa + ml.y * wb;
+    O = O * wa + os * wb;
+    M = Mn;
+  }
+  sm_o[threadIdx.x] = O;
+  if (d == 0) {
+    sm_m[gi] = M;
+    sm_l[gi] = L;
+  }
+  __syncthreads();
+  if (gi != 0) return;
+  float Mt = -INFINITY;
+  for (int i = 0; i < groups; ++i) Mt = fmaxf(Mt, sm_m[i]);
+  float Ls = 0.f, Os = 0.f;
+  for (int i = 0; i < groups; ++i) {
+    const float w = (Mt == -INFINITY) ? 1.f : ex2(sm_m[i] - Mt);
+    Ls += w * sm_l[i];
+    Os += w * sm_o[i * D + d];
+  }
+  store_out(a, (size_t(info.x) + h) * D + d, Os / Ls);
+  if (d == 0 && a.scores) a.row_ml[size_t(info.x) + h] = make_float2(Mt, Ls);
+}
+
+// ------------------------------------------------------------------ accumulated weights
+// weights[b, kh, j] += sum_h exp2(s[h, j] - M[h]) / L[h]; one thread per two tokens, heads in order.
+constexpr int kWeightThreads = 256;
+
+__global__ void __launch_bounds__(kWeightThreads) paged_weights_kernel(const __grid_constant__ PagedLaunch a) {
+  pdl_launch_dependents();
+  pdl_wait_primary();
+  const int b = int(blockIdx.z), kh = int(blockIdx.y);
+  const int j = int(blockIdx.x * kWeightThreads + threadIdx.x) * 2;
+  const int len = min(a.cap, a.seq_lens[b]);
+  if (j >= len) return;
+  const size_t row = size_t(b) * a.Hq + size_t(kh) * a.G;
+  float2 w = make_float2(0.f, 0.f);
+  for (int h = 0; h < a.G; ++h) {
+    const float2 ml = a.row_ml[row + h];
+    const float2 s = *reinterpret_cast<const float2*>(a.scores + (row + h) * size_t(a.cap) + j);
+    const float r = 1.f / ml.y;
+    w.x += ex2(s.x - ml.x) * r;
+    w.y += ex2(s.y - ml.x) * r;
+  }
+  float* dst = a.weights + (size_t(b) * a.Hkv + kh) * size_t(a.cap) + j;
+  dst[0] += w.x;
+  if (j + 1 < len) dst[1] += w.y;
+}
+
+template <int D, bool kI8, int kNT>
+const void* kernel_of() {
+  return reinterpret_cast<const void*>(&paged_attn_kernel<D, kI8, kNT>);
+}
+
+template <int D, bool kI8>
+cudaError_t prepare(int* ctas_per_sm) {
+  int n[2] = {0, 0};
+  for (int i = 0; i < 2; ++i) {
+    const void* fn = i ? kernel_of<D, kI8, 2>() : kernel_of<D, kI8, 1>();
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg<D, kI8>::kSmemBytes));
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n[i], fn, kThr, Cfg<D, kI8>::kSmemBytes);
+    if (e != cudaSuccess) return e;
+    ctas_per_sm[i] = n[i];
+  }
+  return cudaSuccess;
+}
+
+template <int D, bool kI8>
+cudaError_t launch(const PagedLaunch& a, cudaStream_t stream) {
+  constexpr size_t smem = Cfg<D, kI8>::kSmemBytes;
+  return a.GP > 8 ? launch_pdl(paged_attn_kernel<D, kI8, 2>, dim3(a.grid), dim3(kThr), smem, stream, a)
+                  : launch_pdl(paged_attn_kernel<D, kI8, 1>, dim3(a.grid), dim3(kThr), smem, stream, a);
+}
+
+}  // namespace
+
+int paged_tile_keys(bool int8, int D) { return (int8 && D == 64) ? Cfg<64, true>::TK : Cfg<128, false>::TK; }
+
+cudaError_t paged_attn_prepare(bool int8, int D, int (&ctas_per_sm)[2]) {
+  if (int8) return D == 128 ? prepare<128, true>(ctas_per_sm) : prepare<64, true>(ctas_per_sm);
+  return D == 128 ? prepare<128, false>(ctas_per_sm) : prepare<64, false>(ctas_per_sm);
+}
+
+cudaError_t launch_paged_attn(const PagedLaunch& a, cudaStream_t stream) {
+  cudaError_t e;
+  if (a.int8) e = a.D == 128 ? launch<128, true>(a, stream) : launch<64, true>(a, stream);
+  else e = a.D == 128 ? launch<128, false>(a, stream) : launch<64, false>(a, stream);
+  if (e == cudaSuccess && a.part_info)
+    e = launch_pdl(paged_combine_kernel, dim3(a.grid, a.GP), dim3(kCombineThreads), 0, stream, a);
+  if (e == cudaSuccess && a.scores)
+    e = launch_pdl(paged_weights_kernel, dim3((a.cap + 2 * kWeightThreads - 1) / (2 * kWeightThreads), a.Hkv, a.B),
+                   dim3(kWeightThreads), 0, stream, a);
+  return e;
+}
+
+}  // namespace fqkv

@@ -64,6 +64,7 @@ struct DeviceState {
   int max_clusters_f16[2][17] = {};      // fp16 cluster mode: resident clusters per cluster size [D==128][size]
   int max_clusters_qtc[2][17] = {};      // int8 GQA cluster mode: the same for the tensor-core kernel
   int occ_quantize = 0;                  // staged quantizer CTAs per SM
+  int occ_paged[2][2][2] = {};           // paged attention CTAs per SM [int8][D==128][heads > 8]
 };
 DeviceState g_dev[kMaxDevices];
 
@@ -95,6 +96,9 @@ void init_device(DeviceState& ds, int dev) {
   for (int i = 0; i < 2 && e == cudaSuccess; ++i) e = fqkv::decode_kernel_prepare_qtc(false, i ? 128 : 64, &ds.occ_qtc[0][i]);
   for (int i = 0; i < 2 && e == cudaSuccess; ++i) e = fqkv::decode_kernel_prepare_qtc(true, i ? 128 : 64, &ds.occ_qtc[1][i]);
   if (e == cudaSuccess) e = fqkv::quantize_kernel_prepare(&ds.occ_quantize);
+  for (int q = 0; q < 2 && e == cudaSuccess; ++q)
+    for (int i = 0; i < 2 && e == cudaSuccess; ++i) e = fqkv::paged_attn_prepare(q == 1, i ? 128 : 64, ds.occ_paged[q][i]);
+  if (e == cudaSuccess) e = fqkv::evict_prepare();
   if (e != cudaSuccess) return bad(FQKV_ERR_CUDA, cudaGetErrorString(e));
 }
 
@@ -890,6 +894,279 @@ int fqkv_argmax(int32_t model_dtype, const void* logits, int64_t rows, int64_t V
   cudaError_t e = fqkv::launch_argmax(model_dtype == 1, logits, rows, int(V), scratch, idx,
                                       reinterpret_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "argmax launch");
+  return FQKV_OK;
+}
+
+// ------------------------------------------------------------------ paged KV cache
+// The checks every paged entry shares; fills the kernels' view.
+static int paged_cache(const fqkv_paged_kv_t* kv, bool need_lens, fqkv::PagedCache* out) {
+  if (!kv) return fail(FQKV_ERR_INVALID_ARGUMENT, "kv: null paged cache descriptor");
+  if (kv->kv_format != FQKV_KV_F16 && kv->kv_format != FQKV_KV_INT8)
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "kv_format: a paged cache is FQKV_KV_F16 or FQKV_KV_INT8");
+  const bool int8 = kv->kv_format == FQKV_KV_INT8;
+  if (int rc = check_D(kv->D)) return rc;
+  if (kv->page_size < 16 || kv->page_size % 16 != 0)
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "page_size: must be a positive multiple of 16 (got %lld)", (long long)kv->page_size);
+  if (kv->B < 0 || kv->Hkv < 1 || kv->num_pages < 1 || kv->max_pages < 1)
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "negative or zero size (B=%lld Hkv=%lld num_pages=%lld max_pages=%lld)",
+                (long long)kv->B, (long long)kv->Hkv, (long long)kv->num_pages, (long long)kv->max_pages);
+  constexpr int64_t kMax = INT32_MAX;
+  if (kv->num_pages >= kMax || kv->page_size > kMax || kv->Hkv > 65535 || kv->B > 65535 || kv->B * kv->Hkv > 65535 ||
+      kv->max_pages > kMax / kv->page_size)
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "sizes exceed the index range (B * Hkv <= 65535, max_pages * page_size < 2^31)");
+  if (kv->B == 0) return FQKV_OK;
+  if (!kv->k || !kv->v || !kv->block_table || (need_lens && !kv->seq_lens) || (int8 && (!kv->k_scales || !kv->v_scales)))
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (!aligned(kv->k, 16) || !aligned(kv->v, 16) || (int8 && (!aligned(kv->k_scales, 16) || !aligned(kv->v_scales, 16))))
+    return fail(FQKV_ERR_MISALIGNED, "paged K/V and scales must be 16-byte aligned");
+  if (!aligned(kv->block_table, 4) || (need_lens && !aligned(kv->seq_lens, 4)))
+    return fail(FQKV_ERR_MISALIGNED, "block_table / seq_lens must be 4-byte aligned");
+  if (kv->table_stride < 0 || (kv->B > 1 && kv->table_stride < kv->max_pages))
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "block_table: row stride %lld < max_pages", (long long)kv->table_stride);
+  const int elt = int8 ? 1 : 2;
+  // (page, head, token) strides; a dimension of size 1 is never stepped over and gets a legal one
+  int64_t st[2][3];
+  for (int t = 0; t < 2; ++t) {
+    const int64_t* s = t ? kv->v_strides : kv->k_strides;
+    const int64_t size[3] = {kv->num_pages, kv->Hkv, kv->page_size};
+    for (int i = 0; i < 3; ++i) {
+      st[t][i] = size[i] == 1 ? kv->D : s[i];
+      if (st[t][i] < kv->D || st[t][i] * elt >= (int64_t(1) << 40))
+        return fail(FQKV_ERR_INVALID_ARGUMENT, "K/V strides: a row of D elements must not overlap another");
+      if (st[t][i] * elt % 16 != 0) return fail(FQKV_ERR_MISALIGNED, "K/V strides must be multiples of 16 bytes");
+    }
+  }
+  int64_t ss[2][2] = {{0, 0}, {0, 0}};
+  for (int t = 0; t < 2 && int8; ++t) {
+    const int64_t* s = t ? kv->v_scale_strides : kv->k_scale_strides;
+    const int64_t size[2] = {kv->num_pages, kv->Hkv};
+    for (int i = 0; i < 2; ++i) {
+      ss[t][i] = size[i] == 1 ? kv->page_size : s[i];
+      if (ss[t][i] < kv->page_size)
+        return fail(FQKV_ERR_INVALID_ARGUMENT, "scale strides: a page's scales must not overlap another's");
+      if (ss[t][i] % 8 != 0) return fail(FQKV_ERR_MISALIGNED, "scale strides must be multiples of 16 bytes");
+    }
+  }
+  fqkv::PagedCache& c = *out;
+  c.int8 = int8;
+  c.k = const_cast<void*>(kv->k);
+  c.v = const_cast<void*>(kv->v);
+  c.ks = static_cast<__half*>(const_cast<void*>(kv->k_scales));
+  c.vs = static_cast<__half*>(const_cast<void*>(kv->v_scales));
+  c.k_page = st[0][0]; c.k_head = st[0][1]; c.k_tok = st[0][2];
+  c.v_page = st[1][0]; c.v_head = st[1][1]; c.v_tok = st[1][2];
+  c.ks_page = ss[0][0]; c.ks_head = ss[0][1]; c.vs_page = ss[1][0]; c.vs_head = ss[1][1];
+  c.table = reinterpret_cast<const int*>(kv->block_table);
+  c.table_stride = kv->table_stride;
+  c.seq_lens = reinterpret_cast<const int*>(kv->seq_lens);
+  c.num_pages = int(kv->num_pages); c.page = int(kv->page_size);
+  c.B = int(kv->B); c.Hkv = int(kv->Hkv); c.D = int(kv->D);
+  c.cap = int(kv->max_pages * kv->page_size);
+  return FQKV_OK;
+}
+
+// The paged attention's launch shape: head groups, CTAs, and the workspace behind them.
+static int64_t paged_shape(fqkv::PagedLaunch& a, const DeviceState& ds) {
+  a.G = a.Hq / a.Hkv;
+  a.GP = std::min(a.G, fqkv::kPagedMaxHeads);
+  a.groups = (a.G + a.GP - 1) / a.GP;
+  const int tk = fqkv::paged_tile_keys(a.int8, a.D);
+  const int64_t tiles = (int64_t(a.cap) + tk - 1) / tk;  // of a full sequence
+  const int64_t units = int64_t(a.B) * a.Hkv * a.groups;
+  const int64_t resident = int64_t(ds.sm_count) * std::max(1, ds.occ_paged[a.int8][a.D == 128][a.GP > 8]);
+  a.grid = int(std::min(resident, units * tiles));
+  return tiles;
+}
+static size_t pad256(size_t n) { return (n + 255) & ~size_t(255); }
+static size_t paged_parts_bytes(const fqkv::PagedLaunch& a) {
+  return pad256(size_t(a.grid) * sizeof(int4)) + pad256(size_t(a.grid) * 2 * a.GP * sizeof(float2)) +
+         pad256(size_t(a.grid) * 2 * a.GP * a.D * sizeof(float));
+}
+static size_t paged_scores_bytes(const fqkv::PagedLaunch& a) {
+  const size_t rows = size_t(a.B) * a.Hq;
+  return pad256(rows * sizeof(float2)) + rows * a.cap * sizeof(float);
+}
+
+static int paged_heads(int64_t Hq, const fqkv::PagedCache& c) {
+  if (Hq < 1 || Hq % c.Hkv != 0)
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "Hq (%lld) must be a multiple of Hkv (%d)", (long long)Hq, c.Hkv);
+  if (Hq > 65535 || int64_t(c.B) * Hq > INT32_MAX) return fail(FQKV_ERR_INVALID_ARGUMENT, "sizes exceed the index range");
+  // the tiles of all units are numbered in 32 bits
+  const int64_t groups = (Hq / c.Hkv + fqkv::kPagedMaxHeads - 1) / fqkv::kPagedMaxHeads;
+  if (int64_t(c.B) * c.Hkv * groups * (int64_t(c.cap) / 64 + 1) > INT32_MAX)
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "sizes exceed the index range");
+  return FQKV_OK;
+}
+
+size_t fqkv_paged_workspace_bytes(int kv_format, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len, int weights) {
+  if ((kv_format != FQKV_KV_F16 && kv_format != FQKV_KV_INT8) || B < 1 || B > 65535 || Hkv < 1 || Hkv > 65535 || Hq < 1 ||
+      Hq > 65535 || Hq % Hkv != 0 || (D != 64 && D != 128) || max_len < 1 || max_len > INT32_MAX)
+    return 0;
+  DeviceState* ds = nullptr;
+  if (device_state(&ds) != FQKV_OK) return 0;
+  fqkv::PagedLaunch a{};
+  a.int8 = kv_format == FQKV_KV_INT8;
+  a.B = int(B); a.Hq = int(Hq); a.Hkv = int(Hkv); a.D = int(D); a.cap = int(max_len);
+  paged_shape(a, *ds);
+  return paged_parts_bytes(a) + (weights ? paged_scores_bytes(a) : 0);
+}
+
+// K or V pool as (D, page, Hkv, P); box: 128 bytes (fp16) or one row (int8) x `box` tokens.
+static int make_page_map(CUtensorMap* map, const void* base, const fqkv::PagedCache& c, int64_t page, int64_t head,
+                         int64_t tok, int box) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return fail(FQKV_ERR_CUDA, "cuTensorMapEncodeTiled unavailable from the driver");
+  const cuuint64_t elt = c.int8 ? 1 : 2;
+  const cuuint64_t dims[4] = {cuuint64_t(c.D), cuuint64_t(c.page), cuuint64_t(c.Hkv), cuuint64_t(c.num_pages)};
+  const cuuint64_t strides[3] = {cuuint64_t(tok) * elt, cuuint64_t(head) * elt, cuuint64_t(page) * elt};
+  const cuuint32_t boxes[4] = {cuuint32_t(c.int8 ? c.D : 64), cuuint32_t(box), 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(map, c.int8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                   const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   c.int8 && c.D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FQKV_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", int(r));
+  return FQKV_OK;
+}
+
+int fqkv_decode_attn_paged(const fqkv_paged_kv_t* kv, int32_t out_dtype, const void* q, void* o, int64_t Hq,
+                           float* weights, void* workspace, size_t workspace_bytes, fqkv_stream_t stream) {
+  fqkv::PagedCache c{};
+  if (int rc = paged_cache(kv, true, &c)) return rc;
+  if (out_dtype != 0 && out_dtype != 1) return fail(FQKV_ERR_INVALID_ARGUMENT, "out_dtype: 0 (f16) or 1 (bf16)");
+  if (kv->B == 0) return FQKV_OK;
+  if (int rc = paged_heads(Hq, c)) return rc;
+  if (!q || !o) return fail(FQKV_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (!aligned(q, 4) || !aligned(o, 4) || (weights && !aligned(weights, 16)))
+    return fail(FQKV_ERR_MISALIGNED, "q/out must be 4-byte aligned, weights 16-byte");
+  DeviceState* ds = nullptr;
+  if (int rc = device_state(&ds)) return rc;
+  fqkv::PagedLaunch a{};
+  a.int8 = c.int8;
+  a.out_bf16 = out_dtype == 1;
+  a.q = q; a.out = o;
+  a.Ks = c.ks; a.Vs = c.vs;
+  a.ks_page = c.ks_page; a.ks_head = c.ks_head; a.vs_page = c.vs_page; a.vs_head = c.vs_head;
+  a.table = c.table; a.table_stride = c.table_stride; a.seq_lens = c.seq_lens;
+  a.B = c.B; a.Hq = int(Hq); a.Hkv = c.Hkv; a.D = c.D;
+  a.page = c.page; a.cap = c.cap; a.num_pages = c.num_pages;
+  const int64_t tiles = paged_shape(a, *ds);
+  const bool parts = tiles > 1 && a.grid > 1;  // a unit of one tile lies in one CTA
+  const size_t need = (parts ? paged_parts_bytes(a) : 0) + (weights ? paged_scores_bytes(a) : 0);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "workspace: %zu bytes given, %zu needed", workspace ? workspace_bytes : size_t(0),
+                need);
+  if (need && !aligned(workspace, 16)) return fail(FQKV_ERR_MISALIGNED, "workspace must be 16-byte aligned");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (parts) {
+    a.part_info = reinterpret_cast<int4*>(ws);
+    ws += pad256(size_t(a.grid) * sizeof(int4));
+    a.part_ml = reinterpret_cast<float2*>(ws);
+    ws += pad256(size_t(a.grid) * 2 * a.GP * sizeof(float2));
+    a.part_o = reinterpret_cast<float*>(ws);
+    ws += pad256(size_t(a.grid) * 2 * a.GP * a.D * sizeof(float));
+  }
+  if (weights) {
+    a.row_ml = reinterpret_cast<float2*>(ws);
+    a.scores = reinterpret_cast<float*>(ws + pad256(size_t(a.B) * a.Hq * sizeof(float2)));
+    a.weights = weights;
+  }
+  const int tk = fqkv::paged_tile_keys(a.int8, a.D);
+  a.box = 16;
+  while (a.box < tk && a.page % (2 * a.box) == 0) a.box *= 2;
+  if (int rc = make_page_map(&a.tmK, c.k, c, c.k_page, c.k_head, c.k_tok, a.box)) return rc;
+  if (int rc = make_page_map(&a.tmV, c.v, c, c.v_page, c.v_head, c.v_tok, a.box)) return rc;
+  a.sm_scale_log2 = float(1.4426950408889634 / std::sqrt(double(a.D)));
+  a.status = ds->status;
+  a.timeout_ns = g_timeout_ns.load();
+  a.debug_skip_loads = g_debug_skip_loads.load();
+  cudaError_t e = fqkv::launch_paged_attn(a, reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "paged attention launch");
+  return FQKV_OK;
+}
+
+int fqkv_rope_append_paged(const fqkv_paged_kv_t* kv, int32_t model_dtype, const void* qkv, int64_t qkv_row_stride,
+                           const float* cos_table, const float* sin_table, int64_t table_rows, const int32_t* positions,
+                           int64_t position_stride, int32_t axes, const int32_t* axis_map, const int32_t* seq_ids,
+                           const int32_t* slots, void* q_out, int64_t T, int64_t Hq, fqkv_stream_t stream) {
+  fqkv::PagedAppend a{};
+  if (int rc = paged_cache(kv, false, &a.kv)) return rc;
+  if (model_dtype != 0 && model_dtype != 1) return fail(FQKV_ERR_INVALID_ARGUMENT, "model_dtype: 0 (f16) or 1 (bf16)");
+  if (T < 0 || T > INT32_MAX || table_rows < 1 || table_rows > INT32_MAX)
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "bad sizes (T=%lld table_rows=%lld)", (long long)T, (long long)table_rows);
+  if (axes < 1 || axes > 8) return fail(FQKV_ERR_INVALID_ARGUMENT, "axes: 1 to 8 position axes (got %d)", int(axes));
+  if (T == 0) return FQKV_OK;
+  if (kv->B == 0) return fail(FQKV_ERR_INVALID_ARGUMENT, "B: tokens but no sequences");
+  if (int rc = paged_heads(Hq, a.kv)) return rc;
+  if (!seq_ids && T > kv->B)
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "seq_ids: needed for more tokens (%lld) than sequences (%lld)", (long long)T,
+                (long long)kv->B);
+  if (qkv_row_stride < (Hq + 2 * kv->Hkv) * kv->D)
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "qkv_row_stride %lld < (Hq + 2 Hkv) D", (long long)qkv_row_stride);
+  if (axes > 1 && position_stride < T)
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "positions: row stride %lld < T", (long long)position_stride);
+  if (!qkv || !cos_table || !sin_table || !positions || !slots || !q_out || (axes > 1 && !axis_map))
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (!aligned(qkv, 16) || qkv_row_stride % 8 != 0 || !aligned(cos_table, 16) || !aligned(sin_table, 16) || !aligned(q_out, 16))
+    return fail(FQKV_ERR_MISALIGNED, "qkv rows, tables and q_out must be 16-byte aligned");
+  if (!aligned(positions, 4) || !aligned(slots, 4) || (seq_ids && !aligned(seq_ids, 4)) || (axis_map && !aligned(axis_map, 4)))
+    return fail(FQKV_ERR_MISALIGNED, "positions, slots, seq_ids and axis_map must be 4-byte aligned");
+  DeviceState* ds = nullptr;
+  if (int rc = device_state(&ds)) return rc;
+  a.qkv = qkv; a.qkv_stride = qkv_row_stride;
+  a.cos_t = cos_table; a.sin_t = sin_table; a.table_rows = table_rows;
+  a.positions = reinterpret_cast<const int*>(positions); a.pos_stride = position_stride;
+  a.axes = axes;
+  a.axis_map = reinterpret_cast<const int*>(axis_map);
+  a.seq_ids = reinterpret_cast<const int*>(seq_ids);
+  a.slots = reinterpret_cast<const int*>(slots);
+  a.q_out = static_cast<__half*>(q_out);
+  a.T = T; a.Hq = int(Hq);
+  a.status = ds->status;
+  cudaError_t e = fqkv::launch_append_paged(a, model_dtype == 1, reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "paged append launch");
+  return FQKV_OK;
+}
+
+size_t fqkv_evict_workspace_bytes(int64_t B, int64_t Hkv, int64_t max_len, int64_t budget) {
+  if (B < 1 || Hkv < 1 || B > 65535 || Hkv > 65535 || max_len < 1 || budget < 1) return 0;
+  const size_t units = size_t(B) * size_t(Hkv);
+  return pad256(units * sizeof(int2)) + pad256(units * size_t(std::min(max_len, budget)) * sizeof(int));
+}
+
+int fqkv_evict_paged(const fqkv_paged_kv_t* kv, const float* weights, float* weights_out, int32_t* lens_out,
+                     int64_t budget, int64_t recent, void* workspace, size_t workspace_bytes, fqkv_stream_t stream) {
+  fqkv::PagedEvict a{};
+  if (int rc = paged_cache(kv, true, &a.kv)) return rc;
+  if (budget < 1) return fail(FQKV_ERR_INVALID_ARGUMENT, "budget: at least one token stays (got %lld)", (long long)budget);
+  if (recent < 0 || recent > budget)
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "recent: must be in [0, budget] (got %lld)", (long long)recent);
+  if (kv->B == 0) return FQKV_OK;
+  if (!weights || !weights_out || !lens_out) return fail(FQKV_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (!aligned(weights, 16) || !aligned(weights_out, 16) || !aligned(lens_out, 4))
+    return fail(FQKV_ERR_MISALIGNED, "weights must be 16-byte aligned, lens_out 4-byte");
+  const int64_t units = kv->B * kv->Hkv, total = units * int64_t(a.kv.cap);
+  if (weights != weights_out && weights < weights_out + total && weights_out < weights + total)
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "weights_out must be weights itself or not overlap it");
+  // a budget past the capacity evicts nothing; the lists are as long as a sequence at most
+  a.budget = int(std::min<int64_t>(budget, a.kv.cap));
+  a.recent = int(std::min<int64_t>(recent, a.budget));
+  const size_t need = fqkv_evict_workspace_bytes(kv->B, kv->Hkv, a.kv.cap, a.budget);
+  if (!workspace || workspace_bytes < need)
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "workspace: %zu bytes given, %zu needed", workspace ? workspace_bytes : size_t(0),
+                need);
+  if (!aligned(workspace, 16)) return fail(FQKV_ERR_MISALIGNED, "workspace must be 16-byte aligned");
+  DeviceState* ds = nullptr;
+  if (int rc = device_state(&ds)) return rc;
+  a.weights = weights; a.weights_out = weights_out;
+  a.lens_out = reinterpret_cast<int*>(lens_out);
+  a.state = static_cast<int2*>(workspace);
+  a.list = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + pad256(size_t(units) * sizeof(int2)));
+  a.status = ds->status;
+  a.cluster = 1;
+  a.slices = 1;
+  cudaError_t e = fqkv::launch_evict_paged(a, reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "eviction launch");
   return FQKV_OK;
 }
 

@@ -25,6 +25,8 @@ enum : int {
   kDevTimeoutFull = 61,     // consumer waited too long for a tile
   kDevTimeoutEmpty = 62,    // producer waited too long for a free stage
   kDevTimeoutDrain = 63,    // producer could not drain its in-flight copies
+  kDevBadPage = 65,         // a block table names a page outside the pool
+  kDevBadToken = 66,        // a token names a sequence, slot, position or axis outside its range
 };
 
 struct WaitCtl {

@@ -169,6 +169,96 @@ cudaError_t launch_tp_wait(const unsigned long long* counters, int world, unsign
                            unsigned long long* sequence, int* status, unsigned long long timeout_ns,
                            cudaStream_t stream);
 
+// ------------------------------------------------------------------ paged KV cache
+constexpr int kPagedMaxHeads = 16;  // query heads of one KV head that share one pass over its keys
+
+// A paged cache as the kernels see it (the C ABI's fqkv_paged_kv_t, checked): pools [P, Hkv, page, D] with the
+// strides given (elements), scales [P, Hkv, page] (int8) with unit token stride, block table [B, max_pages].
+struct PagedCache {
+  bool int8;
+  void* k;
+  void* v;
+  __half* ks;
+  __half* vs;
+  int64_t k_page, k_head, k_tok, v_page, v_head, v_tok;
+  int64_t ks_page, ks_head, vs_page, vs_head;
+  const int* table;
+  int64_t table_stride;
+  const int* seq_lens;  // [B] (attention, eviction)
+  int num_pages, page, B, Hkv, D;
+  int cap;              // max_pages * page: tokens a sequence can hold
+};
+
+// One call of the paged attention (attn_paged.cu).
+struct PagedLaunch {
+  CUtensorMap tmK, tmV;    // (D, page, Hkv, P), box: 128 bytes (fp16) or a row (int8) x `box` tokens
+  const void* q;           // [B, Hq, D] f16
+  void* out;               // [B, Hq, D] f16, or bf16
+  const __half* Ks;
+  const __half* Vs;
+  int64_t ks_page, ks_head, vs_page, vs_head;
+  const int* table;
+  int64_t table_stride;
+  const int* seq_lens;
+  int B, Hq, Hkv, D;
+  int G, GP, groups;       // query heads per KV head, per unit, units per KV head
+  int page, cap, num_pages, box;
+  int grid;
+  // parts of units that cross a CTA's border; part_info null: none can
+  int4* part_info;         // [grid]: first row, heads, parts of the unit whose first part is this CTA's
+  float2* part_ml;         // [grid * 2][GP]
+  float* part_o;           // [grid * 2][GP][D]
+  // accumulated weights; scores null: not asked for
+  float2* row_ml;          // [B * Hq]
+  float* scores;           // [B * Hq][cap], log2 units
+  float* weights;          // [B, Hkv, cap]
+  float sm_scale_log2;
+  int* status;
+  unsigned long long timeout_ns;
+  int debug_skip_loads;
+  bool int8, out_bf16;
+};
+int paged_tile_keys(bool int8, int D);
+// Resident CTAs per SM of the variants for up to 8 and up to 16 heads per unit.
+cudaError_t paged_attn_prepare(bool int8, int D, int (&ctas_per_sm)[2]);
+cudaError_t launch_paged_attn(const PagedLaunch& a, cudaStream_t stream);
+
+// One call of the paged append (append_paged.cu).
+struct PagedAppend {
+  PagedCache kv;
+  const void* qkv;         // [T, qkv_stride] f16 or bf16
+  int64_t qkv_stride;
+  const float* cos_t;      // [table_rows, D / 2]
+  const float* sin_t;
+  int64_t table_rows;
+  const int* positions;    // [axes, T], row stride pos_stride
+  int64_t pos_stride;
+  const int* axis_map;     // [D / 2] (axes > 1)
+  const int* seq_ids;      // [T], or null: token t is sequence t's
+  const int* slots;        // [T]
+  __half* q_out;           // [T, Hq, D]
+  int64_t T;
+  int Hq, axes;
+  int* status;
+};
+cudaError_t launch_append_paged(const PagedAppend& a, bool bf16, cudaStream_t stream);
+
+// One call of the eviction (evict_paged.cu).
+struct PagedEvict {
+  PagedCache kv;
+  const float* weights;    // [B, Hkv, cap]
+  float* weights_out;      // the same tensor, or another
+  int* lens_out;           // [B]
+  int2* state;             // [B * Hkv]: over budget?, length (workspace)
+  int* list;               // [B * Hkv][budget]: kept tokens in order (workspace)
+  int budget, recent;
+  int cluster;             // selection CTAs per (sequence, KV head)
+  int slices;              // column slices of a row in the move
+  int* status;
+};
+cudaError_t evict_prepare();
+cudaError_t launch_evict_paged(const PagedEvict& a, cudaStream_t stream);
+
 // Log-sum-exp merge of the S_eff partials of every row into out (fp16),
 // chained to the preceding launch by programmatic dependent launch.
 cudaError_t launch_combine(const DecodeLaunch& a, cudaStream_t stream);

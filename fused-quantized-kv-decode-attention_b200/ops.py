@@ -33,6 +33,13 @@ __all__ = [
     "qpt",
     "quant_int4_per_token",
     "workspace_bytes",
+    "decode_attn_gqa_paged",
+    "decode_attn_gqa_int8_paged",
+    "paged_workspace_bytes",
+    "rope_qkv_append_paged",
+    "rope_axes",
+    "evict_kvcache_paged",
+    "evict_workspace_bytes",
 ]
 
 
@@ -488,6 +495,8 @@ DEVICE_STATUS = {
     62: "a decode kernel's producer waited too long for a free pipeline stage",
     63: "a decode kernel could not drain its in-flight copies",
     64: "a tensor-parallel peer's attention outputs never arrived (a rank stopped or fell behind)",
+    65: "a block table named a page outside the pool (the sequence's result is undefined)",
+    66: "an appended token's sequence, slot, position or axis is out of range (the token was not written)",
 }
 
 
@@ -764,3 +773,246 @@ def quant_int4_per_token(X: torch.Tensor):
     292-299): element 2t in the low nibble of byte t.
     """
     return _quantize("quant_int4_per_token", X, True)
+
+
+# ------------------------------------------------------------------ paged KV cache
+def _index_tensor(op: str, name: str, t: torch.Tensor, dev: torch.device) -> None:
+    if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != torch.int32:
+        _fail(op, name, f"{name} must be an int32 tensor on the inputs' device")
+
+
+def _paged_kv(op: str, K, V, Ks, Vs, block_table, seq_lens, dev: torch.device):
+    """Checks a paged cache; returns (packed descriptor, B, Hkv, D, tokens a sequence can hold, int8)."""
+    if K.dim() != 4 or V.shape != K.shape:
+        _fail(op, "shape", "K and V must both be [num_pages, Hkv, page_size, D]")
+    int8 = Ks is not None or Vs is not None
+    key, code = ("int8", torch.int8) if int8 else ("fp16", torch.float16)
+    if K.dtype != code or V.dtype != code:
+        _fail(op, key, f"K and V must be {code} (got {K.dtype}, {V.dtype})")
+    P, Hkv, page, D = K.shape
+    sk, sv = K.stride(), V.stride()
+    if D not in (64, 128):
+        _fail(op, "D", f"head_dim must be 64 or 128 (got {D})")
+    if sk[3] != 1 or sv[3] != 1:
+        _fail(op, "stride", "K and V must be contiguous over D")
+    _index_tensor(op, "block_table", block_table, dev)
+    if block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        _fail(op, "block_table", "block_table must be [B, max_pages] with contiguous rows")
+    B, max_pages = block_table.shape
+    if seq_lens is not None:
+        _index_tensor(op, "seq_lens", seq_lens, dev)
+        if seq_lens.shape != (B,) or (B > 1 and seq_lens.stride(0) != 1):
+            _fail(op, "seq_lens", f"seq_lens must be contiguous [B = {B}]")
+    sks = svs = (0, 0)
+    if int8:
+        _require_cuda(op, K, Ks, Vs)
+        _require_dtype(op, "fp16", torch.float16, Ks=Ks, Vs=Vs)
+        _require_shape(op, "Ks", Ks, (P, Hkv, page))
+        _require_shape(op, "Vs", Vs, (P, Hkv, page))
+        if Ks.stride(2) != 1 or Vs.stride(2) != 1:
+            _fail(op, "stride", "Ks and Vs must be contiguous over a page's tokens")
+        sks, svs = Ks.stride()[:2], Vs.stride()[:2]
+    desc = _native.PAGED_KV.pack(
+        _native.KV_INT8 if int8 else _native.KV_F16, 0, page, P, max_pages, B, Hkv, D, K.data_ptr(), V.data_ptr(),
+        Ks.data_ptr() if int8 else 0, Vs.data_ptr() if int8 else 0, sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], *sks, *svs,
+        block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr() if seq_lens is not None else 0)
+    return desc, B, Hkv, D, max_pages * page, int8
+
+
+def _scratch(op: str, workspace, nbytes: int, dev: torch.device):
+    """The caller's workspace, checked, or a new one from torch's allocator: (pointer, bytes, tensor to keep)."""
+    if workspace is None:
+        if not nbytes:
+            return None, 0, None
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        return workspace.data_ptr(), nbytes, workspace
+    if not isinstance(workspace, torch.Tensor) or workspace.device != dev or not workspace.is_contiguous():
+        _fail(op, "workspace", "workspace must be a contiguous tensor on the inputs' device")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
+
+
+def _slot_weights(op: str, name: str, w, shape, dev: torch.device) -> None:
+    if not isinstance(w, torch.Tensor) or w.device != dev or w.dtype != torch.float32 or not w.is_contiguous() \
+            or w.shape != shape:
+        _fail(op, name, f"{name} must be a contiguous float32 {list(shape)} tensor on the inputs' device")
+
+
+def paged_workspace_bytes(kv_format: str, B: int, Hq: int, Hkv: int, max_len: int, D: int, weights: bool = False) -> int:
+    """Workspace of a paged decode call on the current device; max_len = max_pages * page_size."""
+    fmt = {"fp16": _native.KV_F16, "int8": _native.KV_INT8}[kv_format]
+    return int(_native.lib().fqkv_paged_workspace_bytes(fmt, B, Hq, Hkv, D, max_len, 1 if weights else 0))
+
+
+def evict_workspace_bytes(B: int, Hkv: int, max_len: int, budget: int) -> int:
+    """Workspace of :func:`evict_kvcache_paged`; max_len = max_pages * page_size."""
+    return int(_native.lib().fqkv_evict_workspace_bytes(B, Hkv, max_len, budget))
+
+
+def _decode_paged(op, q, K, V, Ks, Vs, block_table, seq_lens, out, workspace, weights):
+    ts = (q, K, V, block_table, seq_lens)
+    dev = _require_cuda(op, *ts)
+    if q.dim() != 3 or q.dtype != torch.float16 or not q.is_contiguous():
+        _fail(op, "fp16", "q must be a contiguous fp16 [B, Hq, D] tensor")
+    desc, B, Hkv, D, cap, int8 = _paged_kv(op, K, V, Ks, Vs, block_table, seq_lens, dev)
+    Hq = q.shape[1]
+    if q.shape[0] != B or q.shape[2] != D:
+        _fail(op, "shape", f"q has shape {tuple(q.shape)}, expected ({B}, Hq, {D})")
+    if weights is not None:
+        _slot_weights(op, "weights", weights, (B, Hkv, cap), dev)
+    out = _kv_out(op, q, out, q.shape, dev)
+    lib = _native.lib()
+    with _DeviceGuard(dev):
+        need = 0
+        if workspace is None:
+            need = lib.fqkv_paged_workspace_bytes(_native.KV_INT8 if int8 else _native.KV_F16, B, Hq, Hkv, D, cap,
+                                                  0 if weights is None else 1)
+        ws, nb, keep = _scratch(op, workspace, need, dev)
+        rc = lib.fqkv_decode_attn_paged(desc, 1 if out.dtype == torch.bfloat16 else 0, q.data_ptr(), out.data_ptr(), Hq,
+                                        None if weights is None else weights.data_ptr(), ws, nb, _stream(dev))
+    _native.check(rc, f"launch: {op}")
+    return out
+
+
+def decode_attn_gqa_paged(q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, block_table: torch.Tensor,
+                          seq_lens: torch.Tensor, out: torch.Tensor | None = None,
+                          workspace: torch.Tensor | None = None, weights: torch.Tensor | None = None) -> torch.Tensor:
+    """GQA decode over a paged fp16 cache, one length per sequence (one new token each).
+
+    q [B,Hq,D] f16; K/V [num_pages,Hkv,page_size,D] f16 pools, contiguous over D, other strides any multiple of
+    16 bytes (``pool.transpose(1, 2)`` of a [num_pages,page_size,Hkv,D] tensor works); page_size a multiple of 16.
+    ``block_table`` [B,max_pages] int32 names the pages of each sequence, ``seq_lens`` [B] int32 its valid tokens;
+    both are read on the device, so the call can be captured in a CUDA graph.  A sequence of length 0 gives zeros.
+    Table entries past the last page and slots past the last token may hold anything.  A needed page outside the
+    pool is never read: :func:`check_device_status` reports it.
+
+    ``out`` (fp16 or bf16 [B,Hq,D]) and ``workspace`` (``paged_workspace_bytes`` bytes, scratch only; calls that may
+    overlap need one each) are allocated when not given.  ``weights`` [B,Hkv,max_pages*page_size] f32: each token's
+    softmax weight, summed over the query heads of its KV head, is added to it (:func:`evict_kvcache_paged` reads it).
+    """
+    return _decode_paged("decode_attn_gqa_paged", q, K, V, None, None, block_table, seq_lens, out, workspace, weights)
+
+
+def decode_attn_gqa_int8_paged(q, Kq, Vq, Ks, Vs, block_table, seq_lens, out=None, workspace=None,
+                               weights=None) -> torch.Tensor:
+    """As :func:`decode_attn_gqa_paged` over int8 codes [num_pages,Hkv,page_size,D] with f16 scales
+    Ks/Vs [num_pages,Hkv,page_size] (:func:`qpt`'s codes and scales; any query heads per KV head)."""
+    op = "decode_attn_gqa_int8_paged"
+    if Ks is None or Vs is None:
+        _fail(op, "fp16", "Ks and Vs are needed")
+    return _decode_paged(op, q, Kq, Vq, Ks, Vs, block_table, seq_lens, out, workspace, weights)
+
+
+def rope_axes(sections, interleaved: bool = False, device="cuda") -> torch.Tensor:
+    """The position axis of each rotary pair, int32 [sum(sections)]: ``sections[a]`` pairs turn with axis a.
+
+    Contiguous: axis 0's pairs first, then axis 1's, and so on.  Interleaved: pair i < A * sections[i % A] belongs
+    to axis i % A (A axes), the others to axis 0, so every axis gets high and low frequencies.
+    """
+    sections = [int(s) for s in sections]
+    if not sections or min(sections) < 0:
+        raise ValueError(f"rope_axes: sections must be non-negative counts (got {sections})")
+    A = len(sections)
+    if not interleaved:
+        ids = [a for a, s in enumerate(sections) for _ in range(s)]
+    else:
+        ids = [i % A if i < A * sections[i % A] else 0 for i in range(sum(sections))]
+    return torch.tensor(ids, dtype=torch.int32, device=device)
+
+
+def rope_qkv_append_paged(qkv: torch.Tensor, cos_table: torch.Tensor, sin_table: torch.Tensor, positions: torch.Tensor,
+                          slots: torch.Tensor, block_table: torch.Tensor, q_out: torch.Tensor, K: torch.Tensor,
+                          V: torch.Tensor, Ks: torch.Tensor | None = None, Vs: torch.Tensor | None = None,
+                          axes: torch.Tensor | None = None, seq_ids: torch.Tensor | None = None) -> None:
+    """RoPE(q, k) with one or several position axes, q -> fp16, k/v -> their pages, for T tokens in one launch.
+
+    qkv [T,W] (fp16 or bf16, rows 16-byte aligned) holds [q heads | k heads | v heads]; cos_table / sin_table
+    [rows,D/2] float32, one column per rotary pair (i, i + D/2).  ``positions`` int32: [T], or [A,T] with ``axes``
+    (int32 [D/2], see :func:`rope_axes`) saying which row each pair turns with.  Token t goes to slot ``slots[t]``
+    of sequence ``seq_ids[t]`` (None: sequence t); a negative slot is padding and nothing of the token is written.
+    A position need not equal the slot (after an eviction it does not).  q_out [T,Hq,D] fp16; K/V and Ks/Vs as in
+    :func:`decode_attn_gqa_paged` / :func:`decode_attn_gqa_int8_paged`; int8 codes and scales are :func:`qpt`'s of the
+    fp16 row.  fp32 arithmetic, rounded once.  A token out of range is not written and reported by
+    :func:`check_device_status`; two tokens of one call must not share a slot.
+    """
+    op = "rope_qkv_append_paged"
+    dev = _require_cuda(op, qkv, cos_table, sin_table, positions, slots, block_table, q_out, K, V)
+    if qkv.dtype not in (torch.float16, torch.bfloat16):
+        _fail(op, "dtype", "qkv must be fp16 or bf16")
+    if qkv.dim() != 2 or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
+        _fail(op, "shape", "qkv must be [T, W] with contiguous rows")
+    if q_out.dim() != 3 or q_out.dtype != torch.float16 or not q_out.is_contiguous():
+        _fail(op, "fp16", "q_out must be a contiguous fp16 [T, Hq, D] tensor")
+    desc, B, Hkv, D, _, _ = _paged_kv(op, K, V, Ks, Vs, block_table, None, dev)
+    T, Hq = q_out.shape[:2]
+    if q_out.shape[2] != D or qkv.shape[0] != T or qkv.shape[1] < (Hq + 2 * Hkv) * D:
+        _fail(op, "shape", f"qkv must be [T, >= (Hq + 2 Hkv) D] and q_out [T, Hq, {D}] "
+                           f"(got {tuple(qkv.shape)}, {tuple(q_out.shape)})")
+    for name, t in (("cos_table", cos_table), ("sin_table", sin_table)):
+        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != D // 2 or t.shape != cos_table.shape \
+                or not t.is_contiguous():
+            _fail(op, "tables", f"{name} must be contiguous float32 [rows, D/2 = {D // 2}]")
+    _index_tensor(op, "slots", slots, dev)
+    _index_tensor(op, "positions", positions, dev)
+    if slots.shape != (T,) or (T > 1 and slots.stride(0) != 1):
+        _fail(op, "slots", f"slots must be contiguous [T = {T}]")
+    if positions.dim() not in (1, 2) or positions.shape[-1] != T or (T > 1 and positions.stride(-1) != 1):
+        _fail(op, "positions", f"positions must be [T = {T}] or [A, T] with contiguous rows")
+    A = positions.shape[0] if positions.dim() == 2 else 1
+    if A > 1:
+        if axes is None:
+            _fail(op, "axes", "several position axes need axes [D/2]")
+        _index_tensor(op, "axes", axes, dev)
+        if axes.shape != (D // 2,) or not axes.is_contiguous():
+            _fail(op, "axes", f"axes must be contiguous int32 [D/2 = {D // 2}]")
+    if seq_ids is not None:
+        _index_tensor(op, "seq_ids", seq_ids, dev)
+        if seq_ids.shape != (T,) or (T > 1 and seq_ids.stride(0) != 1):
+            _fail(op, "seq_ids", f"seq_ids must be contiguous [T = {T}]")
+    with _DeviceGuard(dev):
+        rc = _native.lib().fqkv_rope_append_paged(
+            desc, 1 if qkv.dtype == torch.bfloat16 else 0, qkv.data_ptr(),
+            qkv.stride(0) if T > 1 else (Hq + 2 * Hkv) * D, cos_table.data_ptr(),
+            sin_table.data_ptr(), cos_table.shape[0], positions.data_ptr(), positions.stride(0) if A > 1 else T, A,
+            axes.data_ptr() if A > 1 else None, None if seq_ids is None else seq_ids.data_ptr(), slots.data_ptr(),
+            q_out.data_ptr(), T, Hq, _stream(dev))
+    _native.check(rc, f"launch: {op}")
+
+
+def evict_kvcache_paged(K: torch.Tensor, V: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                        weights: torch.Tensor, budget: int, recent: int, Ks: torch.Tensor | None = None,
+                        Vs: torch.Tensor | None = None, weights_out: torch.Tensor | None = None,
+                        lens_out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Evict each sequence of a paged cache down to ``budget`` tokens, in place; returns the new lengths [B].
+
+    Every KV head of a longer sequence keeps its newest ``recent`` tokens and, of the others, the
+    ``budget - recent`` with the largest ``weights`` [B,Hkv,max_pages*page_size] f32 (as
+    :func:`decode_attn_gqa_paged` accumulates them; NaN counts as largest, ties go to the lowest index, +inf pins a
+    token).  They keep their order and move to slots 0 .. budget - 1; their rotary positions are inside the keys and do
+    not change.  ``weights_out`` (default: ``weights``, in place) gets the kept tokens' weights and 0 for the freed
+    slots; ``lens_out`` (default: a new tensor; ``seq_lens`` allowed) the new lengths.  Pages shared between
+    sequences must be copied first.  ``workspace``: ``evict_workspace_bytes`` bytes, allocated when not given.
+    """
+    op = "evict_kvcache_paged"
+    dev = _require_cuda(op, K, V, block_table, seq_lens, weights)
+    desc, B, Hkv, D, cap, _ = _paged_kv(op, K, V, Ks, Vs, block_table, seq_lens, dev)
+    _slot_weights(op, "weights", weights, (B, Hkv, cap), dev)
+    if weights_out is None:
+        weights_out = weights
+    else:
+        _slot_weights(op, "weights_out", weights_out, (B, Hkv, cap), dev)
+    if lens_out is None:
+        lens_out = torch.empty_like(seq_lens)
+    else:
+        _index_tensor(op, "lens_out", lens_out, dev)
+        if lens_out.shape != (B,) or (B > 1 and lens_out.stride(0) != 1):
+            _fail(op, "lens_out", f"lens_out must be contiguous [B = {B}]")
+    lib = _native.lib()
+    with _DeviceGuard(dev):
+        need = 0
+        if workspace is None and B:
+            need = lib.fqkv_evict_workspace_bytes(B, Hkv, cap, int(budget))
+        ws, nb, keep = _scratch(op, workspace, need, dev)
+        rc = lib.fqkv_evict_paged(desc, weights.data_ptr(), weights_out.data_ptr(), lens_out.data_ptr(), int(budget),
+                                  int(recent), ws, nb, _stream(dev))
+    _native.check(rc, f"launch: {op}")
+    return lens_out

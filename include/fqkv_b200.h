@@ -59,7 +59,9 @@ const char* fqkv_version(void);
 /* Reads (and, if clear != 0, resets) the in-kernel status word of the current
  * device: 0 = healthy, otherwise the code of the first bounded wait that gave
  * up (61 tile never arrived, 62 stage never freed, 63 copy drain failed,
- * 64 a tensor-parallel peer's attention outputs never arrived).
+ * 64 a tensor-parallel peer's attention outputs never arrived), or of the first
+ * index read on the device that named nothing (paged cache: 65 a page, 66 a
+ * token's sequence, slot, position or axis).
  * Synchronizes with the device. */
 int fqkv_device_status(int* status_out, int clear);
 
@@ -327,6 +329,93 @@ int fqkv_gemv_rope_append(int32_t model_dtype, const void* x, const void* W, con
 size_t fqkv_argmax_scratch_bytes(int64_t rows);
 int fqkv_argmax(int32_t model_dtype, const void* logits, int64_t rows, int64_t V, void* scratch, int64_t* idx,
                 fqkv_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Paged KV cache: pools of pages, a block table, one length per sequence.  No
+ * counterpart in the reference (its caches are dense and share one length).
+ *
+ * Token j of sequence b lies in slot j % page_size of page
+ * block_table[b][j / page_size] of the pools
+ *   k, v [num_pages, Hkv, page_size, D]       f16, or i8 codes
+ *   k_scales, v_scales [num_pages, Hkv, page_size] f16 (FQKV_KV_INT8)
+ * with the (page, head, token) strides given, in elements; D is contiguous,
+ * every stride is a multiple of 16 bytes, and so is every base address.  So a
+ * pool may be stored with tokens outside heads ([num_pages, page_size, Hkv,
+ * D]), or K and V as halves of one tensor.  Scales are contiguous over a
+ * page's tokens.  page_size is any multiple of 16; a dense cache is the case
+ * of one page per sequence.  The stride of a dimension of size 1 is ignored.
+ *
+ * block_table [B, max_pages] (row stride table_stride) and seq_lens [B] are
+ * read on the device, so calls can be captured in a CUDA graph and replayed as
+ * sequences grow.  Lengths are clamped to [0, max_pages * page_size]; table
+ * entries past a sequence's last page, and pool slots past its last token,
+ * may hold anything.  A needed entry outside [0, num_pages) is never
+ * followed: status 65 is recorded (fqkv_device_status) and that sequence's
+ * result is undefined.  B * Hkv <= 65535. */
+typedef struct fqkv_paged_kv {
+  int32_t kv_format;           /* FQKV_KV_F16 or FQKV_KV_INT8 */
+  int32_t reserved;
+  int64_t page_size, num_pages, max_pages, B, Hkv, D;
+  const void* k;               /* written by the append and the eviction */
+  const void* v;
+  const void* k_scales;
+  const void* v_scales;
+  int64_t k_strides[3], v_strides[3];             /* page, head, token */
+  int64_t k_scale_strides[2], v_scale_strides[2]; /* page, head */
+  const int32_t* block_table;
+  int64_t table_stride;
+  const int32_t* seq_lens;     /* attention, eviction */
+} fqkv_paged_kv_t;
+
+/* One new token per sequence: q [B, Hq, D] f16 -> o [B, Hq, D] in out_dtype 0
+ * (f16) or 1 (bf16), softmax over the sequence's own seq_lens[b] tokens (the
+ * new token's k and v are in the cache); query head h reads KV head
+ * h / (Hq/Hkv).  A sequence without tokens gives zeros.  If weights is given
+ * ([B, Hkv, max_pages * page_size] f32, 16-byte aligned), every token's softmax
+ * weight, summed over the query heads of its KV head, is added to it; slots
+ * past the length are left as they are.  Workspace:
+ * fqkv_paged_workspace_bytes(kv_format, B, Hq, Hkv, D, max_pages * page_size,
+ * weights != NULL), scratch only: nothing is kept between calls, and calls
+ * that may overlap need one each. */
+int fqkv_decode_attn_paged(const fqkv_paged_kv_t* kv, int32_t out_dtype, const void* q, void* o, int64_t Hq,
+                           float* weights, void* workspace, size_t workspace_bytes, fqkv_stream_t stream);
+size_t fqkv_paged_workspace_bytes(int kv_format, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len,
+                                  int weights);
+
+/* Rotary embedding, fp16 cast of q and cache append of T tokens.  qkv [T,
+ * qkv_row_stride] (model_dtype 0 = f16, 1 = bf16; rows 16-byte aligned) holds
+ * [q heads | k heads | v heads].  Pair i of a q or k head -- dimensions i and
+ * i + D/2 -- is turned by the angle in row positions[axis_map[i]][t], column i
+ * of cos_table / sin_table [table_rows, D/2] f32; `axes` position rows, axis_map
+ * [D/2] (not read when axes is 1).  q -> q_out [T, Hq, D] f16; k and v -> slot
+ * slots[t] of sequence seq_ids[t] (NULL: sequence t), as f16, or as the codes and scale
+ * that fqkv_quantize_int8_per_token gives for the f16 row.  All arithmetic is
+ * fp32, rounded once to f16.  A token with a negative slot is padding:
+ * nothing of it is written, q_out included.  One whose sequence, slot or
+ * position is out of range is not written either and records status 66 (65: its page), an
+ * axis out of range records 66 and its pairs are undefined.  Two tokens of one
+ * call must not share a slot.  seq_lens is not used.  Extends
+ * fqkv_rope_qkv_append, whose rounding follows transformers' in the model dtype. */
+int fqkv_rope_append_paged(const fqkv_paged_kv_t* kv, int32_t model_dtype, const void* qkv, int64_t qkv_row_stride,
+                           const float* cos_table, const float* sin_table, int64_t table_rows, const int32_t* positions,
+                           int64_t position_stride, int32_t axes, const int32_t* axis_map, const int32_t* seq_ids,
+                           const int32_t* slots, void* q_out, int64_t T, int64_t Hq, fqkv_stream_t stream);
+
+/* Eviction by accumulated attention weight.  Each KV head of a sequence with
+ * more than `budget` tokens keeps its newest `recent` and, of the others, the
+ * budget - recent of the largest weights[b][kh][j] (f32 [B, Hkv, max_pages *
+ * page_size]; NaN counts as largest; ties go to the lowest index; +inf pins a
+ * token).  What stays keeps its order and moves to slots 0 .. budget - 1 of the
+ * sequence's pages, in place; weights_out (weights itself, or a tensor of the
+ * same shape) gets the kept tokens' weights and 0 for the freed slots up to the
+ * old length, lens_out[b] (seq_lens itself allowed) the new length.  Other
+ * sequences keep their rows (weights_out gets their weights).  Pages that
+ * several sequences share must be copied first.  Workspace:
+ * fqkv_evict_workspace_bytes(B, Hkv, max_pages * page_size, budget), scratch
+ * only. */
+int fqkv_evict_paged(const fqkv_paged_kv_t* kv, const float* weights, float* weights_out, int32_t* lens_out,
+                     int64_t budget, int64_t recent, void* workspace, size_t workspace_bytes, fqkv_stream_t stream);
+size_t fqkv_evict_workspace_bytes(int64_t B, int64_t Hkv, int64_t max_len, int64_t budget);
 
 /* ------------------------------------------------------------------------
  * Tensor-parallel decode: attention fused with the all-gather of its outputs.
