@@ -84,12 +84,12 @@ __global__ void __launch_bounds__(kAppendThreads) append_paged_kernel(const __gr
     if (threadIdx.x == 0) atomicCAS(a.status, kDevOk, kDevBadToken);
     return;
   }
-  const int page = a.kv.table[int64_t(seq) * a.kv.table_stride + slot / a.kv.page];
+  const int page = a.kv.table[int64_t(seq) * a.kv.table_stride + a.kv.page_div.div(slot)];
   if (unsigned(page) >= unsigned(a.kv.num_pages)) {
     if (threadIdx.x == 0) atomicCAS(a.status, kDevOk, kDevBadPage);
     return;
   }
-  const int off = slot % a.kv.page;
+  const int off = a.kv.page_div.mod(slot);
 
   // cosines and sines of pairs 8j .. 8j + 7
   float c[8], s[8];

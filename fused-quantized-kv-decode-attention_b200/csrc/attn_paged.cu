@@ -48,7 +48,7 @@ constexpr int kMergeHeads = 4;     // heads merged per epilogue pass
 
 template <int D, bool kI8>
 struct Cfg {
-  static constexpr int KPW = (kI8 && D == 64) ? 32 : 16;  // keys of a tile per consumer warp
+  static constexpr int KPW = kI8 ? 32 : 16;    // keys of a tile per consumer warp
   static constexpr int TK = kWarps * KPW;                 // keys per tile
   static constexpr int kBlocks = kI8 ? 1 : D / 64;        // column blocks of a tile (128-byte fp16 rows)
   static constexpr int RB = kI8 ? D : 128;                // bytes of a row of a column block
@@ -56,7 +56,11 @@ struct Cfg {
   static constexpr int kTileBytes = kBlocks * kBlockBytes;  // K (or V) of one tile
   static constexpr int kScaleBytes = kI8 ? 2 * TK : 0;
   static constexpr int kStageBytes = 2 * kTileBytes + (kI8 ? 1024 : 0);  // scales in a 1 KB tail: tiles stay aligned
-  static constexpr int kCtas = D == 128 ? (kI8 ? 3 : 2) : (kI8 ? 3 : 4);
+  // fp16: as many CTAs as fit beside three stages (3 CTAs of two stages at D = 128 measured within 1 %).
+  // int8: 32 keys per warp, so that two independent 16-key chains cover each other's latency, and registers for
+  // them: B = 64, 16K, D = 128 301 us; 16 keys per warp and 3 CTAs 316 us (4 CTAs spill: 350 us), 32 keys and 3 CTAs
+  // of two stages 354 us (spills).
+  static constexpr int kCtas = D == 128 ? 2 : (kI8 ? 3 : 4);
   static constexpr int kStages = 3;
   static constexpr size_t kRingBytes = size_t(kStages) * kStageBytes;
   static constexpr size_t kBarBytes = 2 * kStages * sizeof(uint64_t);
@@ -76,16 +80,28 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
-// Byte offset of 16-byte chunk `c` of row `row` in a column block written with the swizzle of its row width.
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+// One arrival on `bar` when this thread's cp.async copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Byte offset of 16-byte chunk `chunk` of row `row` of a tile written with the swizzle of its row width: the
+// chunk's number XOR the row's place in the swizzle atom.  For a lane's row and chunk parity, the offset of chunk
+// 2i + parity is that of `parity` XOR 32 i within a column block (tiles are 1024-byte aligned), so a lane needs
+// one logic operation per ldmatrix.
 template <int RB>
 __device__ __forceinline__ uint32_t blk_off(int row, int c) {
   if constexpr (RB == 128) return uint32_t(row * 128 + ((c ^ (row & 7)) << 4));
   else return uint32_t(row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
 }
+// Address of chunk 2i + parity from the address `at` of chunk `parity`.
 template <int D, bool kI8>
-__device__ __forceinline__ uint32_t tile_off(int row, int chunk) {
-  if constexpr (kI8) return blk_off<Cfg<D, kI8>::RB>(row, chunk);
-  else return uint32_t((chunk >> 3) * Cfg<D, kI8>::kBlockBytes) + blk_off<128>(row, chunk & 7);
+__device__ __forceinline__ uint32_t chunk_at(uint32_t at, int i) {
+  constexpr int kPer = Cfg<D, kI8>::RB / 32;  // chunk pairs per column block
+  return (at ^ uint32_t((i % kPer) * 32)) + uint32_t((i / kPer) * Cfg<D, kI8>::kBlockBytes);
 }
 
 // ------------------------------------------------------------------ the line of tiles
@@ -210,7 +226,7 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], kI8 ? 1 + 32 : 1);  // int8: the producer's lanes fetch the scales
       mbar_init(&empty[s], kWarps);
     }
     abort_flag = 0;
@@ -233,15 +249,16 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
     if (!a.debug_skip_loads) {
       const int br = a.box;             // keys per box
       const int nb = C::TK / br;        // boxes per tile: 1, 2, 4 or 8
-      constexpr int kKinds = kI8 ? 4 : 2 * C::kBlocks;  // copies per box
+      constexpr int kKinds = 2 * C::kBlocks;  // copies per box
       const int job_box = lane / kKinds, kind = lane % kKinds;
+      const int sc_key = (lane % (C::TK / 8)) * 8;  // int8: 8 scales of K (the lower lanes) or of V
       int it = 0;
       bool ok = true;
       while (ok && walk.next(p)) {
         const int* row = a.table + int64_t(p.b) * a.table_stride;
         const int first = p.t0 * nb;                                   // boxes counted from the sequence's start
         const int last = min(p.t1 * nb, (p.len + br - 1) / br);        // boxes that hold tokens
-        auto page_of = [&](int box) { return box < last ? row[(int64_t(box) * br) / a.page] : 0; };
+        auto page_of = [&](int box) { return box < last ? row[a.page_div.div(box * br)] : 0; };
         int ids = page_of(first + lane), ids_next = page_of(first + 32 + lane), at = 0;
         for (int t = p.t0; t < p.t1 && ok; ++t, ++it, at += nb) {
           if (at == 32) {  // nb divides 32
@@ -259,29 +276,33 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
             }
           }
           const int boxes = min(nb, last - t * nb);  // a box past the last token is not fetched
-          if (lane == 0)
-            mbar_arrive_expect_tx(&full[st], uint32_t(boxes) * br * uint32_t(2 * C::kBlocks * C::RB + (kI8 ? 4 : 0)));
+          if (lane == 0) mbar_arrive_expect_tx(&full[st], uint32_t(boxes) * br * uint32_t(2 * C::kBlocks * C::RB));
           __syncwarp();
-          int id = __shfl_sync(0xffffffffu, ids, (at + job_box) & 31);
+          uint8_t* stage = smem + size_t(st) * C::kStageBytes;
+          const int id = __shfl_sync(0xffffffffu, ids, (at + job_box) & 31);
           if (job_box < boxes) {
-            const int tok = int((int64_t(t) * C::TK + job_box * br) % a.page);
+            const int tok = a.page_div.mod(t * C::TK + job_box * br);
             const bool known = unsigned(id) < unsigned(a.num_pages);
             if (!known && kind == 0) atomicCAS(a.status, kDevOk, kDevBadPage);
-            uint8_t* stage = smem + size_t(st) * C::kStageBytes;
-            if (kI8 && kind >= 2) {
-              // a number outside the pool: some scales, for the zero codes of its keys
-              const int pg = known ? id : 0;
-              const __half* src = kind == 2 ? a.Ks + int64_t(pg) * a.ks_page + int64_t(p.kh) * a.ks_head + tok
-                                            : a.Vs + int64_t(pg) * a.vs_page + int64_t(p.kh) * a.vs_head + tok;
-              bulk_g2s(stage + 2 * C::kTileBytes + (kind - 2) * C::kScaleBytes + job_box * br * 2, src, uint32_t(br) * 2,
-                       &full[st]);
-            } else {
-              const bool is_v = kI8 ? kind == 1 : kind >= C::kBlocks;
-              const int blk = kI8 ? 0 : kind % C::kBlocks;
-              uint8_t* dst = stage + (is_v ? C::kTileBytes : 0) + blk * C::kBlockBytes + job_box * br * C::RB;
-              // outside the pool the copy unit writes zeros and reads nothing
-              tma_load_4d(dst, is_v ? &a.tmV : &a.tmK, blk * 64, tok, p.kh, known ? id : a.num_pages, &full[st]);
+            const bool is_v = kind >= C::kBlocks;
+            const int blk = kind % C::kBlocks;
+            uint8_t* dst = stage + (is_v ? C::kTileBytes : 0) + blk * C::kBlockBytes + job_box * br * C::RB;
+            // outside the pool the copy unit writes zeros and reads nothing
+            tma_load_4d(dst, is_v ? &a.tmV : &a.tmK, blk * 64, tok, p.kh, known ? id : a.num_pages, &full[st]);
+          }
+          if constexpr (kI8) {
+            // 16-byte pieces of scales, not copies of a box's 32 to 256 bytes: the copy unit's requests are what
+            // bounds small pages (D = 64, 16-token pages, B = 64, 4K: 77 us with, 72 us without)
+            const int sc_box = sc_key / br;
+            const int sid = __shfl_sync(0xffffffffu, ids, (at + sc_box) & 31);
+            if (sc_box < boxes) {
+              const int pg = unsigned(sid) < unsigned(a.num_pages) ? sid : 0;  // some scales for zero codes
+              const int tok = a.page_div.mod(t * C::TK + sc_key);
+              const __half* src = lane < C::TK / 8 ? a.Ks + pg * a.ks_page + p.kh * a.ks_head + tok
+                                                   : a.Vs + pg * a.vs_page + p.kh * a.vs_head + tok;
+              cp_async16(stage + 2 * C::kTileBytes + lane * 16, src);
             }
+            cp_async_arrive(&full[st]);
           }
         }
       }
@@ -299,17 +320,24 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
   const int t4 = lane & 3;
   const int mi = lane >> 3;  // ldmatrix matrix of this lane
   const int rr = lane & 7;   // and row in it
+  const int r0 = warp * C::KPW;  // this warp's first key of a tile
+  // this lane's row and chunk parity in the ldmatrix of K (keys by 8, then chunks) and of V (chunks, then keys)
+  const uint32_t k_off = blk_off<C::RB>(r0 + ((mi >> 1) << 3) + rr, mi & 1);
+  const uint32_t v_off = blk_off<C::RB>(r0 + ((mi & 1) << 3) + rr, mi >> 1);
   const uint32_t ring = smem_u32(smem);
   const int ct = threadIdx.x;
   bool alive = true;
   int it = 0;
 
-  // sequences without tokens: zeros
+  // sequences without tokens: zeros, and no parts
   for (int b = int(blockIdx.x); b < a.B; b += int(gridDim.x))
-    if (a.seq_lens[b] <= 0)
+    if (a.seq_lens[b] <= 0) {
       for (int i = ct; i < a.Hq * D; i += 32 * kWarps) store_out(a, size_t(b) * a.Hq * D + i, 0.f);
+      const int units = a.Hkv * a.groups;
+      if (a.unit_info)
+        for (int i = ct; i < units; i += 32 * kWarps) a.unit_info[b * units + i] = make_int2(0, 0);
+    }
 
-  int4 info = make_int4(0, 0, 0, 0);
   while (walk.next(p)) {
     const int h0 = p.kh * a.G + p.grp * a.GP;
     const int gvalid = min(a.GP, a.G - p.grp * a.GP);
@@ -362,7 +390,6 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
       auto tile = [&](auto mask_tag) {
         constexpr bool kMask = decltype(mask_tag)::value;
         constexpr int NJ = C::KPW / 8;
-        const int r0 = warp * C::KPW;
         // ---- S = Q K^T
         float sc[NJ][4];
 #pragma unroll
@@ -373,12 +400,12 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
         };
 #pragma unroll
         for (int kb = 0; kb < C::KPW / 16; ++kb) {
-          const int row = r0 + 16 * kb + ((mi >> 1) << 3) + rr;
+          const uint32_t at = sk + k_off + uint32_t(16 * kb * C::RB);
           if constexpr (!kI8) {
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
               uint32_t b0, b1, b2, b3;
-              ldmatrix_x4(sk + tile_off<D, kI8>(row, 2 * kk + (mi & 1)), b0, b1, b2, b3);
+              ldmatrix_x4(chunk_at<D, kI8>(at, kk), b0, b1, b2, b3);
               mma_s(sc[2 * kb], kk, b0, b1);
               mma_s(sc[2 * kb + 1], kk, b2, b3);
             }
@@ -386,7 +413,7 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
 #pragma unroll
             for (int kk = 0; kk < D / 16; kk += 2) {
               uint32_t b[4];  // (keys 0-7, chunk kk), (keys 0-7, kk + 1), (keys 8-15, kk), (keys 8-15, kk + 1)
-              ldmatrix_x4(sk + tile_off<D, kI8>(row, kk + (mi & 1)), b[0], b[1], b[2], b[3]);
+              ldmatrix_x4(chunk_at<D, kI8>(at, kk / 2), b[0], b[1], b[2], b[3]);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const uint32_t x = b[i] ^ 0x80808080u;
@@ -488,7 +515,7 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
               const float* s2 = &sc[2 * kb + i][2 * nt];
               pb[nt][i] = kI8 ? pack_half2(s2[0] * vs[2 * kb + i][0], s2[1] * vs[2 * kb + i][1]) : pack_half2(s2[0], s2[1]);
             }
-          const int row = r0 + 16 * kb + ((mi & 1) << 3) + rr;
+          const uint32_t at = sv + v_off + uint32_t(16 * kb * C::RB);
           if constexpr (!kI8) {
             // The slots past the last token may hold anything, and 0 * inf is NaN: they are masked to zero.
             uint32_t vm0 = 0xffffffffu, vm1 = 0xffffffffu;
@@ -500,7 +527,7 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
 #pragma unroll
             for (int dd = 0; dd < D / 16; ++dd) {
               uint32_t v0, v1, v2, v3;  // (keys 0-7, dims 0-7), (keys 8-15, dims 0-7), (0-7, 8-15), (8-15, 8-15)
-              ldmatrix_x4_trans(sv + tile_off<D, kI8>(row, 2 * dd + (mi >> 1)), v0, v1, v2, v3);
+              ldmatrix_x4_trans(chunk_at<D, kI8>(at, dd), v0, v1, v2, v3);
               if constexpr (kMask) {
                 v0 &= vm0;
                 v1 &= vm1;
@@ -516,7 +543,7 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
 #pragma unroll
             for (int dd = 0; dd < D / 16; dd += 2) {
               uint32_t v[4];  // (keys 0-7, chunk dd), (keys 8-15, dd), (0-7, dd + 1), (8-15, dd + 1)
-              ldmatrix_x4_trans(sv + tile_off<D, kI8>(row, dd + (mi >> 1)), v[0], v[1], v[2], v[3]);
+              ldmatrix_x4_trans(chunk_at<D, kI8>(at, dd / 2), v[0], v[1], v[2], v[3]);
 #pragma unroll
               for (int i = 0; i < 4; ++i) v[i] ^= 0x80808080u;
 #pragma unroll
@@ -593,81 +620,165 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
       }
       named_bar_sync(1, 32 * kWarps);
     }
-    if (p.t0 == 0 && p.t1 < p.nt)  // this CTA holds the unit's first part; the merge starts here
-      info = make_int4(int(row_base), gvalid, 1 + (p.nt - p.t1 + walk.per - 1) / walk.per, 0);
+    // the CTA that a unit begins in says in how many parts it comes, and from which CTA on
+    if (p.t0 == 0 && ct == 0 && a.unit_info) {
+      const int more = p.nt - p.t1;
+      a.unit_info[(p.b * a.Hkv + p.kh) * a.groups + p.grp] =
+          make_int2(int(blockIdx.x), more ? 1 + (more + walk.per - 1) / walk.per : 0);
+    }
   }
-  if (ct == 0 && a.part_info) a.part_info[blockIdx.x] = info;
 }
 
-// ------------------------------------------------------------------ merge of the units that cross a border
-// CTA c: the unit whose first part is CTA c's (part_info[c]); its parts are slot 1 of CTA c and slot 0 of the
-// following ones, merged in that order.  blockIdx.y: a head.  Thread: one dimension of one group of parts.
-constexpr int kCombineThreads = 256;
+// ------------------------------------------------------------------ the rest of a call
+// One launch after the attention.  Its first blocks merge the units that came in parts: part s of a unit is
+// slot 1 of CTA info.x (s = 0) or slot 0 of CTA info.x + s, always taken in this order.  The other blocks, if
+// weights are accumulated, add the softmax weights of a stretch of tokens of one (sequence, KV head); they merge
+// the parts' maxima and sums for themselves, so that nothing waits for a third launch.
+constexpr int kFinishThreads = 256;
+constexpr int kFinishWarps = kFinishThreads / 32;
 
-__global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const __grid_constant__ PagedLaunch a) {
-  pdl_launch_dependents();
-  pdl_wait_primary();
-  __shared__ float sm_o[kCombineThreads], sm_m[kCombineThreads / 64], sm_l[kCombineThreads / 64];
-  const int4 info = a.part_info[blockIdx.x];  // row of the unit's first head, heads, parts
-  const int h = int(blockIdx.y);
-  if (h >= info.y) return;
-  const int D = a.D, groups = kCombineThreads / D;
-  const int gi = threadIdx.x / D, d = threadIdx.x - gi * D;
-  float M = -INFINITY, L = 0.f, O = 0.f;
-#pragma unroll 8
-  for (int s = gi; s < info.z; s += groups) {
-    const size_t slot = (size_t(blockIdx.x) + s) * 2 + (s == 0 ? 1 : 0);
-    const float2 ml = a.part_ml[slot * a.GP + h];
-    const float os = a.part_o[(slot * a.GP + h) * D + d];
+// A unit's parts, none if it was finished in one CTA.  (Lengths that another stream changes during a call could leave
+// an entry unwritten; then nothing is followed.)
+__device__ __forceinline__ int2 parts_of(const PagedLaunch& a, int unit) {
+  const int2 info = a.unit_info[unit];
+  const bool legal = info.x >= 0 && info.y >= 0 && info.x < a.grid && info.y <= a.grid - info.x;
+  return legal ? info : make_int2(0, 0);
+}
+__device__ __forceinline__ size_t part_slot(const int2& info, int s) { return (size_t(info.x) + s) * 2 + (s == 0 ? 1 : 0); }
+
+// Maximum and sum of a head over a unit's parts, by one warp; every lane gets both.
+__device__ __forceinline__ float2 merge_ml(const PagedLaunch& a, const int2& info, int h) {
+  const int lane = threadIdx.x & 31;
+  float M = -INFINITY, L = 0.f;
+  for (int s = lane; s < info.y; s += 32) {
+    const float2 ml = a.part_ml[part_slot(info, s) * a.GP + h];
     const float Mn = fmaxf(M, ml.x);
-    const float wa = (Mn == -INFINITY) ? 1.f : ex2(M - Mn);
-    const float wb = (Mn == -INFINITY) ? 1.f : ex2(ml.x - Mn);
-    L = L * wa + ml.y * wb;
-    O = O * wa + os * wb;
+    L = (Mn == -INFINITY) ? L + ml.y : L * ex2(M - Mn) + ml.y * ex2(ml.x - Mn);
     M = Mn;
   }
-  sm_o[threadIdx.x] = O;
-  if (d == 0) {
-    sm_m[gi] = M;
-    sm_l[gi] = L;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    const float Mo = __shfl_xor_sync(0xffffffffu, M, off), Lo = __shfl_xor_sync(0xffffffffu, L, off);
+    const float Mn = fmaxf(M, Mo);
+    L = (Mn == -INFINITY) ? L + Lo : L * ex2(M - Mn) + Lo * ex2(Mo - Mn);
+    M = Mn;
   }
-  __syncthreads();
-  if (gi != 0) return;
-  float Mt = -INFINITY;
-  for (int i = 0; i < groups; ++i) Mt = fmaxf(Mt, sm_m[i]);
-  float Ls = 0.f, Os = 0.f;
-  for (int i = 0; i < groups; ++i) {
-    const float w = (Mt == -INFINITY) ? 1.f : ex2(sm_m[i] - Mt);
-    Ls += w * sm_l[i];
-    Os += w * sm_o[i * D + d];
-  }
-  store_out(a, (size_t(info.x) + h) * D + d, Os / Ls);
-  if (d == 0 && a.scores) a.row_ml[size_t(info.x) + h] = make_float2(Mt, Ls);
+  return make_float2(M, L);
 }
 
-// ------------------------------------------------------------------ accumulated weights
-// weights[b, kh, j] += sum_h exp2(s[h, j] - M[h]) / L[h]; one thread per two tokens, heads in order.
-constexpr int kWeightThreads = 256;
+// Merge of `a.merge_heads` heads of one unit, from head h0: the block's warps are shared out over the heads, the warps
+// of a head take its parts in turn (4 dimensions per lane; D = 64: half a warp per part), each with its own running
+// maximum, so that a part's numbers and its maximum are fetched together.
+template <int D>
+__device__ void merge_unit(const PagedLaunch& a, const int2& info, int unit, int h0, float* sm_o, float2* sm_ml) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int grp = unit % a.groups, bk = unit / a.groups;
+  const int heads = min(min(a.merge_heads, a.GP - h0), a.G - grp * a.GP - h0);  // of this block
+  const size_t row0 = size_t(bk / a.Hkv) * a.Hq + size_t(bk % a.Hkv) * a.G + size_t(grp) * a.GP + h0;
+  constexpr int kLanes = D / 4, kPer = 32 / kLanes;       // lanes per part, parts per warp and step
+  const int share = max(1, kFinishWarps / a.merge_heads);  // warps per head
+  const int heads_at_once = kFinishWarps / share;
+  const int sub = (warp % share) * kPer + lane / kLanes;  // this lane's place among those of its head and dimension
+  const int d = (lane % kLanes) * 4;
+  for (int hb = 0; hb < heads; hb += heads_at_once) {
+    const int h = hb + warp / share;
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (h < heads) {
+#pragma unroll 4
+      for (int s = sub; s < info.y; s += share * kPer) {
+        const size_t row = part_slot(info, s) * a.GP + h0 + h;
+        const float2 ml = a.part_ml[row];
+        const float4 o = *reinterpret_cast<const float4*>(a.part_o + row * D + d);
+        const float Mn = fmaxf(M, ml.x);
+        const float wa = Mn == -INFINITY ? 1.f : ex2(M - Mn), wb = Mn == -INFINITY ? 1.f : ex2(ml.x - Mn);
+        M = Mn;
+        L = L * wa + ml.y * wb;
+        acc.x = acc.x * wa + o.x * wb;
+        acc.y = acc.y * wa + o.y * wb;
+        acc.z = acc.z * wa + o.z * wb;
+        acc.w = acc.w * wa + o.w * wb;
+      }
+    }
+    const int mine = (warp / share) * share * kPer + sub;
+    *reinterpret_cast<float4*>(sm_o + mine * D + d) = acc;
+    if (d == 0) sm_ml[mine] = make_float2(M, L);
+    __syncthreads();
+    for (int i = threadIdx.x; i < min(heads_at_once, heads - hb) * D; i += kFinishThreads) {
+      const int hh = i / D, e = i - hh * D, first = hh * share * kPer;
+      float Mt = -INFINITY, Lt = 0.f, Ot = 0.f;
+      for (int k = 0; k < share * kPer; ++k) Mt = fmaxf(Mt, sm_ml[first + k].x);
+      for (int k = 0; k < share * kPer; ++k) {
+        const float2 ml = sm_ml[first + k];
+        const float w = Mt == -INFINITY ? 1.f : ex2(ml.x - Mt);
+        Lt += w * ml.y;
+        Ot += w * sm_o[(first + k) * D + e];
+      }
+      store_out(a, (row0 + hb + hh) * D + e, Ot / Lt);
+    }
+    __syncthreads();
+  }
+}
 
-__global__ void __launch_bounds__(kWeightThreads) paged_weights_kernel(const __grid_constant__ PagedLaunch a) {
+// weights[b, kh, j] += sum_h exp2(s[h, j] - M[h]) / L[h], heads in order; 4 tokens per thread.
+constexpr int kWeightTokens = 4 * kFinishThreads;
+
+__device__ void add_weights(const PagedLaunch& a, int block, float2* sm_ml) {
+  const int chunks = (a.cap + kWeightTokens - 1) / kWeightTokens;
+  const int bk = block / chunks, b = bk / a.Hkv, kh = bk - b * a.Hkv;
+  const int len = min(a.cap, a.seq_lens[b]);
+  const int j0 = (block - bk * chunks) * kWeightTokens;
+  if (j0 >= len) return;
+  const size_t row = size_t(b) * a.Hq + size_t(kh) * a.G;
+  const int j = j0 + 4 * int(threadIdx.x);
+  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int h0 = 0; h0 < a.G; h0 += kPagedMaxHeads) {  // the heads of a unit at a time
+    const int nh = min(kPagedMaxHeads, a.G - h0);
+    const int unit = bk * a.groups + h0 / a.GP;
+    const int2 info = a.unit_info ? parts_of(a, unit) : make_int2(0, 0);
+    for (int h = threadIdx.x >> 5; h < nh; h += kFinishWarps) {
+      const float2 ml = info.y ? merge_ml(a, info, h) : a.row_ml[row + h0 + h];
+      if ((threadIdx.x & 31) == 0) sm_ml[h] = make_float2(ml.x, 1.f / ml.y);
+    }
+    __syncthreads();
+    if (j < len) {
+#pragma unroll 4
+      for (int h = 0; h < nh; ++h) {
+        // cap and j are multiples of 4; what lies past the length is read but not used
+        const float4 s = *reinterpret_cast<const float4*>(a.scores + (row + h0 + h) * size_t(a.cap) + j);
+        const float2 ml = sm_ml[h];
+        w[0] += ex2(s.x - ml.x) * ml.y;
+        w[1] += ex2(s.y - ml.x) * ml.y;
+        w[2] += ex2(s.z - ml.x) * ml.y;
+        w[3] += ex2(s.w - ml.x) * ml.y;
+      }
+    }
+    __syncthreads();
+  }
+  if (j >= len) return;
+  float* dst = a.weights + (size_t(b) * a.Hkv + kh) * size_t(a.cap) + j;
+  if (j + 4 <= len) {
+    float4 old = *reinterpret_cast<const float4*>(dst);
+    *reinterpret_cast<float4*>(dst) = make_float4(old.x + w[0], old.y + w[1], old.z + w[2], old.w + w[3]);
+  } else {
+    for (int i = 0; i < len - j; ++i) dst[i] += w[i];
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(const __grid_constant__ PagedLaunch a) {
+  __shared__ __align__(16) float sm_o[kFinishThreads * 4];
+  __shared__ float2 sm_ml[kPagedMaxHeads];  // merge: two per warp
   pdl_launch_dependents();
   pdl_wait_primary();
-  const int b = int(blockIdx.z), kh = int(blockIdx.y);
-  const int j = int(blockIdx.x * kWeightThreads + threadIdx.x) * 2;
-  const int len = min(a.cap, a.seq_lens[b]);
-  if (j >= len) return;
-  const size_t row = size_t(b) * a.Hq + size_t(kh) * a.G;
-  float2 w = make_float2(0.f, 0.f);
-  for (int h = 0; h < a.G; ++h) {
-    const float2 ml = a.row_ml[row + h];
-    const float2 s = *reinterpret_cast<const float2*>(a.scores + (row + h) * size_t(a.cap) + j);
-    const float r = 1.f / ml.y;
-    w.x += ex2(s.x - ml.x) * r;
-    w.y += ex2(s.y - ml.x) * r;
+  if (int(blockIdx.x) >= a.merge_blocks) {
+    add_weights(a, int(blockIdx.x) - a.merge_blocks, sm_ml);
+    return;
   }
-  float* dst = a.weights + (size_t(b) * a.Hkv + kh) * size_t(a.cap) + j;
-  dst[0] += w.x;
-  if (j + 1 < len) dst[1] += w.y;
+  const int per_unit = (a.GP + a.merge_heads - 1) / a.merge_heads;
+  const int unit = int(blockIdx.x) / per_unit;
+  const int2 info = parts_of(a, unit);
+  if (info.y) merge_unit<D>(a, info, unit, (int(blockIdx.x) - unit * per_unit) * a.merge_heads, sm_o, sm_ml);
 }
 
 template <int D, bool kI8, int kNT>
@@ -697,7 +808,7 @@ cudaError_t launch(const PagedLaunch& a, cudaStream_t stream) {
 
 }  // namespace
 
-int paged_tile_keys(bool int8, int D) { return (int8 && D == 64) ? Cfg<64, true>::TK : Cfg<128, false>::TK; }
+int paged_tile_keys(bool int8) { return int8 ? Cfg<128, true>::TK : Cfg<128, false>::TK; }
 
 cudaError_t paged_attn_prepare(bool int8, int D, int (&ctas_per_sm)[2]) {
   if (int8) return D == 128 ? prepare<128, true>(ctas_per_sm) : prepare<64, true>(ctas_per_sm);
@@ -708,11 +819,12 @@ cudaError_t launch_paged_attn(const PagedLaunch& a, cudaStream_t stream) {
   cudaError_t e;
   if (a.int8) e = a.D == 128 ? launch<128, true>(a, stream) : launch<64, true>(a, stream);
   else e = a.D == 128 ? launch<128, false>(a, stream) : launch<64, false>(a, stream);
-  if (e == cudaSuccess && a.part_info)
-    e = launch_pdl(paged_combine_kernel, dim3(a.grid, a.GP), dim3(kCombineThreads), 0, stream, a);
-  if (e == cudaSuccess && a.scores)
-    e = launch_pdl(paged_weights_kernel, dim3((a.cap + 2 * kWeightThreads - 1) / (2 * kWeightThreads), a.Hkv, a.B),
-                   dim3(kWeightThreads), 0, stream, a);
+  if (e == cudaSuccess && (a.unit_info || a.scores)) {
+    const int chunks = a.scores ? (a.cap + kWeightTokens - 1) / kWeightTokens : 0;
+    const dim3 grid(unsigned(a.merge_blocks) + unsigned(a.B * a.Hkv) * unsigned(chunks));
+    e = a.D == 128 ? launch_pdl(paged_finish_kernel<128>, grid, dim3(kFinishThreads), 0, stream, a)
+                   : launch_pdl(paged_finish_kernel<64>, grid, dim3(kFinishThreads), 0, stream, a);
+  }
   return e;
 }
 

@@ -962,6 +962,7 @@ static int paged_cache(const fqkv_paged_kv_t* kv, bool need_lens, fqkv::PagedCac
   c.num_pages = int(kv->num_pages); c.page = int(kv->page_size);
   c.B = int(kv->B); c.Hkv = int(kv->Hkv); c.D = int(kv->D);
   c.cap = int(kv->max_pages * kv->page_size);
+  c.page_div = fqkv::FastDiv(c.page);
   return FQKV_OK;
 }
 
@@ -970,7 +971,7 @@ static int64_t paged_shape(fqkv::PagedLaunch& a, const DeviceState& ds) {
   a.G = a.Hq / a.Hkv;
   a.GP = std::min(a.G, fqkv::kPagedMaxHeads);
   a.groups = (a.G + a.GP - 1) / a.GP;
-  const int tk = fqkv::paged_tile_keys(a.int8, a.D);
+  const int tk = fqkv::paged_tile_keys(a.int8);
   const int64_t tiles = (int64_t(a.cap) + tk - 1) / tk;  // of a full sequence
   const int64_t units = int64_t(a.B) * a.Hkv * a.groups;
   const int64_t resident = int64_t(ds.sm_count) * std::max(1, ds.occ_paged[a.int8][a.D == 128][a.GP > 8]);
@@ -979,7 +980,7 @@ static int64_t paged_shape(fqkv::PagedLaunch& a, const DeviceState& ds) {
 }
 static size_t pad256(size_t n) { return (n + 255) & ~size_t(255); }
 static size_t paged_parts_bytes(const fqkv::PagedLaunch& a) {
-  return pad256(size_t(a.grid) * sizeof(int4)) + pad256(size_t(a.grid) * 2 * a.GP * sizeof(float2)) +
+  return pad256(size_t(a.B) * a.Hkv * a.groups * sizeof(int2)) + pad256(size_t(a.grid) * 2 * a.GP * sizeof(float2)) +
          pad256(size_t(a.grid) * 2 * a.GP * a.D * sizeof(float));
 }
 static size_t paged_scores_bytes(const fqkv::PagedLaunch& a) {
@@ -1049,7 +1050,8 @@ int fqkv_decode_attn_paged(const fqkv_paged_kv_t* kv, int32_t out_dtype, const v
   a.ks_page = c.ks_page; a.ks_head = c.ks_head; a.vs_page = c.vs_page; a.vs_head = c.vs_head;
   a.table = c.table; a.table_stride = c.table_stride; a.seq_lens = c.seq_lens;
   a.B = c.B; a.Hq = int(Hq); a.Hkv = c.Hkv; a.D = c.D;
-  a.page = c.page; a.cap = c.cap; a.num_pages = c.num_pages;
+  a.cap = c.cap; a.num_pages = c.num_pages;
+  a.page_div = c.page_div;
   const int64_t tiles = paged_shape(a, *ds);
   const bool parts = tiles > 1 && a.grid > 1;  // a unit of one tile lies in one CTA
   const size_t need = (parts ? paged_parts_bytes(a) : 0) + (weights ? paged_scores_bytes(a) : 0);
@@ -1059,21 +1061,28 @@ int fqkv_decode_attn_paged(const fqkv_paged_kv_t* kv, int32_t out_dtype, const v
   if (need && !aligned(workspace, 16)) return fail(FQKV_ERR_MISALIGNED, "workspace must be 16-byte aligned");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   if (parts) {
-    a.part_info = reinterpret_cast<int4*>(ws);
-    ws += pad256(size_t(a.grid) * sizeof(int4));
+    const int units = a.B * a.Hkv * a.groups;
+    a.unit_info = reinterpret_cast<int2*>(ws);
+    ws += pad256(size_t(units) * sizeof(int2));
     a.part_ml = reinterpret_cast<float2*>(ws);
     ws += pad256(size_t(a.grid) * 2 * a.GP * sizeof(float2));
     a.part_o = reinterpret_cast<float*>(ws);
     ws += pad256(size_t(a.grid) * 2 * a.GP * a.D * sizeof(float));
+    // Few units have many parts each: a block per head, its eight warps on that head's parts.  Many units have few
+    // parts: a block per unit, its warps shared out over the heads.
+    a.merge_heads = units * a.GP <= 2 * ds->sm_count ? 1 : a.GP;
+    a.merge_blocks = units * ((a.GP + a.merge_heads - 1) / a.merge_heads);
   }
   if (weights) {
     a.row_ml = reinterpret_cast<float2*>(ws);
     a.scores = reinterpret_cast<float*>(ws + pad256(size_t(a.B) * a.Hq * sizeof(float2)));
     a.weights = weights;
   }
-  const int tk = fqkv::paged_tile_keys(a.int8, a.D);
+  if (weights && int64_t(a.B) * a.Hkv * (a.cap / 1024 + 1) > INT32_MAX / 2)
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "sizes exceed the index range");
+  const int tk = fqkv::paged_tile_keys(a.int8);
   a.box = 16;
-  while (a.box < tk && a.page % (2 * a.box) == 0) a.box *= 2;
+  while (a.box < tk && c.page % (2 * a.box) == 0) a.box *= 2;
   if (int rc = make_page_map(&a.tmK, c.k, c, c.k_page, c.k_head, c.k_tok, a.box)) return rc;
   if (int rc = make_page_map(&a.tmV, c.v, c, c.v_page, c.v_head, c.v_tok, a.box)) return rc;
   a.sm_scale_log2 = float(1.4426950408889634 / std::sqrt(double(a.D)));

@@ -196,7 +196,7 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 
 // Page of position p, or -1 (recorded) when the table names none of the pool's.
 __device__ __forceinline__ int page_at(const PagedEvict& a, const int* row, int p) {
-  const int id = row[p / a.kv.page];
+  const int id = row[a.kv.page_div.div(p)];
   if (unsigned(id) < unsigned(a.kv.num_pages)) return id;
   atomicCAS(a.status, kDevOk, kDevBadPage);
   return -1;
@@ -220,7 +220,7 @@ __device__ void move_rows(const PagedEvict& a, const int* list, const int* row, 
   const uint32_t my = smem_u32(ring) + tid * 16;
   auto at = [&](int p, int col) -> uint8_t* {
     const int pg = page_at(a, row, p);
-    return pg < 0 ? nullptr : base + pg * page_stride + (p % a.kv.page) * tok_stride + 16 * col;
+    return pg < 0 ? nullptr : base + pg * page_stride + a.kv.page_div.mod(p) * tok_stride + 16 * col;
   };
   unsigned got = 0;  // which pieces of the chunks in flight were fetched, 4 bits per stage
   auto fetch = [&](int c) {
@@ -283,8 +283,8 @@ __device__ void move_scalars(const PagedEvict& a, const int* list, const int* ro
       if (a.kv.int8) {
         const int pg = page_at(a, row, s);
         if (pg >= 0) {
-          ks = a.kv.ks[pg * a.kv.ks_page + kh * a.kv.ks_head + s % a.kv.page];
-          vs = a.kv.vs[pg * a.kv.vs_page + kh * a.kv.vs_head + s % a.kv.page];
+          ks = a.kv.ks[pg * a.kv.ks_page + kh * a.kv.ks_head + a.kv.page_div.mod(s)];
+          vs = a.kv.vs[pg * a.kv.vs_page + kh * a.kv.vs_head + a.kv.page_div.mod(s)];
           sc = true;
         }
       }
@@ -294,8 +294,8 @@ __device__ void move_scalars(const PagedEvict& a, const int* list, const int* ro
       wo[p] = x;
       const int pg = sc ? page_at(a, row, p) : -1;
       if (pg >= 0) {
-        a.kv.ks[pg * a.kv.ks_page + kh * a.kv.ks_head + p % a.kv.page] = ks;
-        a.kv.vs[pg * a.kv.vs_page + kh * a.kv.vs_head + p % a.kv.page] = vs;
+        a.kv.ks[pg * a.kv.ks_page + kh * a.kv.ks_head + a.kv.page_div.mod(p)] = ks;
+        a.kv.vs[pg * a.kv.vs_page + kh * a.kv.vs_head + a.kv.page_div.mod(p)] = vs;
       }
     }
   }

@@ -172,6 +172,22 @@ cudaError_t launch_tp_wait(const unsigned long long* counters, int world, unsign
 // ------------------------------------------------------------------ paged KV cache
 constexpr int kPagedMaxHeads = 16;  // query heads of one KV head that share one pass over its keys
 
+// Division of 0 <= n < 2^31 by a fixed 1 <= d < 2^31: n / d = (mulhi(n, mul) + n) >> shift with
+// shift = ceil(log2 d), mul = floor(2^32 (2^shift - d) / d) + 1 (Granlund and Montgomery, "Division by
+// invariant integers using multiplication", 1994; mulhi(n, mul) + n < 2^32 for these n).
+struct FastDiv {
+  uint32_t d, mul, shift;
+  FastDiv() = default;
+  explicit FastDiv(int div) : d(uint32_t(div)), shift(0) {
+    while ((uint64_t(1) << shift) < d) ++shift;
+    mul = uint32_t((((uint64_t(1) << shift) - d) << 32) / d + 1);
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ int div(int n) const { return int((__umulhi(uint32_t(n), mul) + uint32_t(n)) >> shift); }
+  __device__ __forceinline__ int mod(int n) const { return n - div(n) * int(d); }
+#endif
+};
+
 // A paged cache as the kernels see it (the C ABI's fqkv_paged_kv_t, checked): pools [P, Hkv, page, D] with the
 // strides given (elements), scales [P, Hkv, page] (int8) with unit token stride, block table [B, max_pages].
 struct PagedCache {
@@ -187,6 +203,7 @@ struct PagedCache {
   const int* seq_lens;  // [B] (attention, eviction)
   int num_pages, page, B, Hkv, D;
   int cap;              // max_pages * page: tokens a sequence can hold
+  FastDiv page_div;
 };
 
 // One call of the paged attention (attn_paged.cu).
@@ -202,23 +219,25 @@ struct PagedLaunch {
   const int* seq_lens;
   int B, Hq, Hkv, D;
   int G, GP, groups;       // query heads per KV head, per unit, units per KV head
-  int page, cap, num_pages, box;
+  int cap, num_pages, box;
+  FastDiv page_div;
   int grid;
-  // parts of units that cross a CTA's border; part_info null: none can
-  int4* part_info;         // [grid]: first row, heads, parts of the unit whose first part is this CTA's
+  // parts of units that cross a CTA's border; unit_info null: none can
+  int2* unit_info;         // [B * Hkv * groups]: the CTA of the first part, the number of parts (0: none)
   float2* part_ml;         // [grid * 2][GP]
   float* part_o;           // [grid * 2][GP][D]
   // accumulated weights; scores null: not asked for
   float2* row_ml;          // [B * Hq]
   float* scores;           // [B * Hq][cap], log2 units
   float* weights;          // [B, Hkv, cap]
+  int merge_blocks, merge_heads;  // blocks of the second launch that merge parts, and the heads of each
   float sm_scale_log2;
   int* status;
   unsigned long long timeout_ns;
   int debug_skip_loads;
   bool int8, out_bf16;
 };
-int paged_tile_keys(bool int8, int D);
+int paged_tile_keys(bool int8);
 // Resident CTAs per SM of the variants for up to 8 and up to 16 heads per unit.
 cudaError_t paged_attn_prepare(bool int8, int D, int (&ctas_per_sm)[2]);
 cudaError_t launch_paged_attn(const PagedLaunch& a, cudaStream_t stream);
