@@ -1172,8 +1172,6 @@ int fqkv_evict_paged(const fqkv_paged_kv_t* kv, const float* weights, float* wei
   a.state = static_cast<int2*>(workspace);
   a.list = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + pad256(size_t(units) * sizeof(int2)));
   a.status = ds->status;
-  a.cluster = 1;
-  a.slices = 1;
   cudaError_t e = fqkv::launch_evict_paged(a, reinterpret_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "eviction launch");
   return FQKV_OK;

@@ -5,17 +5,20 @@
 // order and moves to slots 0 .. budget - 1 of the sequence's own pages; its weights move along and the freed
 // slots' weights become 0.  Sequences of at most `budget` tokens are left as they are.
 //
-// Two launches.  The selection: one thread-block cluster per (sequence, KV head); every CTA counts its slice of
-// the weights into 2048 bins of the order-preserving 32-bit key, the cluster adds the bins through
-// distributed shared memory and narrows the key digit by digit (11, 11 and 10 bits) to the smallest one kept;
-// a last pass numbers the kept tokens in order and writes their list.  Bound by latency: five passes over
-// 4 bytes per token, from L2 after the first.
+// Two launches.  The selection: one CTA, or one thread-block cluster for long caches, per (sequence, KV head).  The
+// weights' order-preserving 32-bit keys are counted into 2048 bins by their first 11 bits; the bin of the last
+// key kept is found, its keys set apart, and the other 11 and 10 bits found among those; then the kept tokens are
+// numbered in order and listed.  Bound by instructions and latency (128 selections of 4096 from 16K tokens:
+// 15 us, 58 % of the issue slots); in a cluster the CTAs add their few used bins to the first one's by
+// distributed-shared-memory atomics, integers, so the order does not matter.
 //
-// The move: bound by HBM, 2 x the kept rows.  In place, and the list is ascending with list[p] >= p: a row's
+// The move: bound by HBM, 2 x the kept rows (48 sequences of 16K -> 4096, D = 128, fp16: 1.65 GB in 369 us, selection
+// included).  In place, and the list is ascending with list[p] >= p: a row's
 // destination is at or before its source.  One CTA moves one column slice of K (or V) of one (sequence, KV
 // head), chunk by chunk in list order; a chunk is written only after it and all earlier chunks were read, and a
 // chunk's writes end below the next chunk's first source, so reading ahead is free.  Slices make enough CTAs for
-// few sequences.  The chunks before the first gap are not touched.
+// few sequences.  The chunks before the first gap are not touched.  32 KB chunks, three in flight: chunks of
+// 16 KB are as fast for 16 x 16K and slower for long moves (4 x 100000 -> 50000: 555 us instead of 457 us).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -28,10 +31,10 @@
 namespace fqkv {
 namespace {
 
-constexpr int kSelThreads = 512;
+constexpr int kSelThreads = 1024;
 constexpr int kBins = 2048;
 
-// Larger weight, larger key; -0 as +0; every NaN above +inf.
+// Larger weight, larger key; -0 as +0; every NaN above +inf.  No weight has the key 0.
 __device__ __forceinline__ uint32_t weight_key(float w) {
   if (isnan(w)) return 0xffffffffu;
   const uint32_t u = __float_as_uint(w + 0.f);
@@ -44,6 +47,10 @@ __device__ __forceinline__ uint32_t ld_dsmem_u32(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ void red_dsmem_add(uint32_t addr, uint32_t v) {
+  asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
 // Inclusive sum over the block in thread order; every thread also gets the total.
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, uint32_t* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -54,136 +61,246 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, 
   }
   if (lane == 31) warp_sums[warp] = v;
   __syncthreads();
-  uint32_t before = 0, all = 0;
+  // every warp scans the 32 warps' sums
+  static_assert(kSelThreads == 1024, "one lane per warp");
+  uint32_t all = warp_sums[lane];
 #pragma unroll
-  for (int w = 0; w < kSelThreads / 32; ++w) {
-    const uint32_t s = warp_sums[w];
-    if (w < warp) before += s;
-    all += s;
+  for (int off = 1; off < 32; off <<= 1) {
+    const uint32_t u = __shfl_up_sync(0xffffffffu, all, off);
+    if (lane >= off) all += u;
   }
+  const uint32_t before = warp ? __shfl_sync(0xffffffffu, all, warp - 1) : 0u;
+  all = __shfl_sync(0xffffffffu, all, 31);
   __syncthreads();  // warp_sums may be written again
   *total = all;
   return before + v;
 }
 
-// Cluster of gridDim-independent size `a.cluster` per (sequence, KV head).
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_constant__ PagedEvict a) {
-  __shared__ uint32_t hist[kBins];
-  __shared__ uint32_t warp_sums[kSelThreads / 32];
-  __shared__ uint32_t sel_bin, sel_above, my_counts[2];
-  pdl_launch_dependents();
-  pdl_wait_primary();
-  const int C = a.cluster;
-  const int rank = int(blockIdx.x) % C;
-  const int unit = int(blockIdx.x) / C;
-  const int tid = threadIdx.x;
-  const int n = max(0, min(a.kv.cap, a.kv.seq_lens[unit / a.kv.Hkv]));
-  const bool over = n > a.budget;
-  if (rank == 0 && tid == 0) a.state[unit] = make_int2(over ? 1 : 0, n);
-  if (!over) return;  // the whole cluster
+constexpr int kMost = 16 * kSelThreads;         // tokens of a step; a slice of one step stays in registers
+constexpr int kCand = 4096;                     // keys that share the first digit and fit in shared memory
 
-  const float* w = a.weights + size_t(unit) * a.kv.cap;
-  int* list = a.list + size_t(unit) * a.budget;
-  const int m = n - a.recent, k = a.budget - a.recent;  // keep k of the first m, and the rest
-  for (int i = rank * kSelThreads + tid; i < a.recent; i += C * kSelThreads) list[k + i] = m + i;
-  if (k == 0) return;  // the whole cluster
+struct SelectShared {
+  uint32_t hist[2][kBins];  // the next digit's bins are cleared while this one's are in use
+  uint32_t cand[kCand];
+  uint32_t warp_sums[kSelThreads / 32];
+  uint32_t sel[2];          // the digit chosen, and how many keys lie in the bins above it
+  uint32_t cands, larger;   // this slice's keys in the first digit's bin, and above it
+  uint32_t counts[2];
+};
 
-  const int per = ((m + C - 1) / C + 3) & ~3;
-  const int s0 = min(m, rank * per), s1 = min(m, s0 + per);
+// One slice is read three times: for the first digit's bins, to pick out the keys in the bin chosen (the two other
+// digits then look at those alone, unless there are more than kCand of them), and for the list.
+// kMine: consecutive tokens of one thread per step (4 where a slice has no more than 4096: the selection and move of one sequence
+// of 2112 tokens take 18.4 us, with 16 tokens per thread 20.5 us).
+template <int kMine, bool kOneStep>
+__device__ void select_tokens(const PagedEvict& a, const float* w, int* list, int rank, int s0, int s1, int k,
+                              SelectShared& sm) {
+  constexpr int kStep = kMine * kSelThreads;
+  const int C = a.cluster, tid = threadIdx.x, lane = tid & 31;
+  // f(this thread's first token, its keys) for every step; every thread takes part in every step.  Tokens past the
+  // slice have key 0, below every weight's (a key of 0 would be a NaN with the sign bit, and those are mapped away).
+  auto fetch = [&](int i0, uint32_t (&key)[kMine]) {
+#pragma unroll
+    for (int q = 0; q < kMine; q += 4) {  // a row of weights is whole 16-byte pieces
+      const float4 x = i0 + q < s1 ? *reinterpret_cast<const float4*>(w + i0 + q) : make_float4(0.f, 0.f, 0.f, 0.f);
+      key[q] = weight_key(x.x);
+      key[q + 1] = weight_key(x.y);
+      key[q + 2] = weight_key(x.z);
+      key[q + 3] = weight_key(x.w);
+    }
+    if (i0 + kMine > s1) {
+#pragma unroll
+      for (int q = 0; q < kMine; ++q)
+        if (i0 + q >= s1) key[q] = 0u;
+    }
+  };
+  uint32_t cached[kOneStep ? kMine : 1];
+  if constexpr (kOneStep) fetch(s0 + kMine * tid, cached);
+  auto steps = [&](auto&& f) {
+    if constexpr (kOneStep) {
+      f(s0 + kMine * tid, cached);
+    } else {
+      for (int c0 = s0; c0 < s1; c0 += kStep) {
+        uint32_t key[kMine];
+        fetch(c0 + kMine * tid, key);
+        f(c0 + kMine * tid, key);
+      }
+    }
+  };
 
   // ---- the smallest key kept, digit by digit
   uint32_t prefix = 0, mask = 0, need = uint32_t(k);
+  for (int i = tid; i < kBins; i += kSelThreads) sm.hist[0][i] = 0;
+  if (tid == 0) sm.cands = sm.larger = 0;
+  if (C > 1) cluster_sync_all();
+  else __syncthreads();
+  bool few = false;  // the keys in the first digit's bin are in sm.cand
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
     const uint32_t digit = pass == 2 ? 1023u : 2047u;
-    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+    uint32_t* hist = sm.hist[pass & 1];
+    if (few) {
+      for (int i = tid; i < int(sm.cands); i += kSelThreads) {
+        const uint32_t key = sm.cand[i];
+        if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & digit], 1u);
+      }
+    } else {
+      steps([&](int, const uint32_t(&key)[kMine]) {
+#pragma unroll
+        for (int q = 0; q < kMine; ++q)
+          if (key[q] != 0u && (key[q] & mask) == prefix) atomicAdd(&hist[(key[q] >> shift) & digit], 1u);
+      });
+    }
+    for (int i = tid; i < kBins; i += kSelThreads) sm.hist[(pass + 1) & 1][i] = 0;
     __syncthreads();
-    for (int i = s0 + tid; i < s1; i += kSelThreads) {
-      const uint32_t key = weight_key(w[i]);
-      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & digit], 1u);
+    if (C > 1) {  // the first CTA gets the others' counts: few of the bins are in use
+      if (rank != 0)
+        for (int i = tid; i < kBins; i += kSelThreads)
+          if (hist[i]) red_dsmem_add(dsmem_addr(smem_u32(&hist[i]), 0), hist[i]);
+      cluster_sync_all();
     }
-    cluster_sync_all();
-    // thread tid: bins 2047 - 4 tid down to 2044 - 4 tid, summed over the cluster
-    constexpr int kPer = kBins / kSelThreads;
-    uint32_t cnt[kPer], sum = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int bin = kBins - 1 - (kPer * tid + i);
-      uint32_t v = 0;
-      for (int r = 0; r < C; ++r) v += ld_dsmem_u32(dsmem_addr(smem_u32(&hist[bin]), r));
-      cnt[i] = v;
-      sum += v;
-    }
-    uint32_t total;
-    uint32_t above = block_scan(sum, warp_sums, &total) - sum;  // in the bins above this thread's
-    if (above < need && need <= above + sum) {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        if (above < need && need <= above + cnt[i]) {
-          sel_bin = uint32_t(kBins - 1 - (kPer * tid + i));
-          sel_above = above;
-        }
-        above += cnt[i];
+    if (rank == 0) {
+      // thread tid: bins 2047 - 2 tid and 2046 - 2 tid
+      const uint32_t hi = hist[kBins - 1 - 2 * tid], lo = hist[kBins - 2 - 2 * tid];
+      uint32_t total;
+      const uint32_t above = block_scan(hi + lo, sm.warp_sums, &total) - hi - lo;
+      if (above < need && need <= above + hi + lo) {
+        const bool first = need <= above + hi;
+        sm.sel[0] = uint32_t(kBins - (first ? 1 : 2) - 2 * tid);
+        sm.sel[1] = first ? above : above + hi;
       }
     }
-    cluster_sync_all();  // sel_* are set; every CTA has read the bins
-    need -= sel_above;
-    prefix |= sel_bin << shift;
+    uint32_t bin, over;
+    if (C > 1) {
+      cluster_sync_all();
+      bin = ld_dsmem_u32(dsmem_addr(smem_u32(&sm.sel[0]), 0));
+      over = ld_dsmem_u32(dsmem_addr(smem_u32(&sm.sel[1]), 0));
+    } else {
+      __syncthreads();
+      bin = sm.sel[0];
+      over = sm.sel[1];
+    }
+    // sel is set again behind the next pass's barriers, which every reader has to reach first
+    need -= over;
+    prefix |= bin << shift;
     mask |= digit << shift;
-    __syncthreads();  // all have read sel_* before the next pass sets them
+    if (pass == 0) {
+      steps([&](int, const uint32_t(&key)[kMine]) {
+        uint32_t mine = 0, above = 0;
+#pragma unroll
+        for (int q = 0; q < kMine; ++q) {
+          mine += (key[q] >> 21) == bin && key[q] != 0u;
+          above += (key[q] >> 21) > bin;
+        }
+        above = __reduce_add_sync(0xffffffffu, above);
+        uint32_t incl = mine;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const uint32_t u = __shfl_up_sync(0xffffffffu, incl, off);
+          if (lane >= off) incl += u;
+        }
+        uint32_t at = 0;
+        if (lane == 31) {
+          atomicAdd(&sm.larger, above);
+          at = atomicAdd(&sm.cands, incl);
+        }
+        at = __shfl_sync(0xffffffffu, at, 31) + incl - mine;
+#pragma unroll
+        for (int q = 0; q < kMine; ++q)
+          if ((key[q] >> 21) == bin && key[q] != 0u) {
+            if (at < kCand) sm.cand[at] = key[q];
+            ++at;
+          }
+      });
+      __syncthreads();
+      few = sm.cands <= kCand;
+    }
   }
 
   // ---- numbers of larger and equal keys in the slices before this CTA's
-  uint32_t gt = 0, eq = 0;
-  for (int i = s0 + tid; i < s1; i += kSelThreads) {
-    const uint32_t key = weight_key(w[i]);
-    gt += key > prefix;
-    eq += key == prefix;
-  }
-  uint32_t tot_gt, tot_eq;
-  block_scan(gt, warp_sums, &tot_gt);
-  block_scan(eq, warp_sums, &tot_eq);
-  if (tid == 0) {
-    my_counts[0] = tot_gt;
-    my_counts[1] = tot_eq;
-  }
-  cluster_sync_all();
   uint32_t gt_before = 0, eq_before = 0;
-  for (int r = 0; r < rank; ++r) {
-    gt_before += ld_dsmem_u32(dsmem_addr(smem_u32(&my_counts[0]), r));
-    eq_before += ld_dsmem_u32(dsmem_addr(smem_u32(&my_counts[1]), r));
-  }
-  cluster_sync_all();  // no CTA leaves while its counts are read
-
-  // ---- the list, in order: 4 consecutive tokens per thread and step
-  for (int c0 = s0; c0 < s1; c0 += 4 * kSelThreads) {
-    uint32_t key[4], mine = 0;  // equal keys in the high half, larger ones in the low half
-    const int i0 = c0 + 4 * tid;
+  if (C > 1) {
+    uint32_t gt = 0, eq = 0;
+    if (few) {
+      for (int i = tid; i < int(sm.cands); i += kSelThreads) {
+        gt += sm.cand[i] > prefix;
+        eq += sm.cand[i] == prefix;
+      }
+    } else {
+      steps([&](int, const uint32_t(&key)[kMine]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      key[i] = i0 + i < s1 ? weight_key(w[i0 + i]) : 0u;
-      if (i0 + i < s1) mine += (key[i] > prefix ? 1u : 0u) + (key[i] == prefix ? 0x10000u : 0u);
+        for (int q = 0; q < kMine; ++q) {
+          gt += (key[q] >> 21) == (prefix >> 21) && key[q] > prefix;
+          eq += key[q] == prefix;
+        }
+      });
     }
-    uint32_t total;
-    const uint32_t before = block_scan(mine, warp_sums, &total) - mine;
-    uint32_t g = gt_before + (before & 0xffffu), e = eq_before + (before >> 16);
+    uint32_t tot_gt, tot_eq;
+    block_scan(gt, sm.warp_sums, &tot_gt);
+    block_scan(eq, sm.warp_sums, &tot_eq);
+    if (tid == 0) {
+      sm.counts[0] = sm.larger + tot_gt;
+      sm.counts[1] = tot_eq;
+    }
+    cluster_sync_all();
+    for (int r = 0; r < rank; ++r) {
+      gt_before += ld_dsmem_u32(dsmem_addr(smem_u32(&sm.counts[0]), r));
+      eq_before += ld_dsmem_u32(dsmem_addr(smem_u32(&sm.counts[1]), r));
+    }
+    cluster_sync_all();  // no CTA leaves while its counts are read
+  }
+
+  // ---- the list, in order (a step's counts: larger keys in the low half, equal ones in the high half, at most
+  // 16384 each)
+  steps([&](int i0, const uint32_t(&key)[kMine]) {
+    uint32_t mine = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i0 + i >= s1) continue;
-      const bool is_gt = key[i] > prefix, is_eq = key[i] == prefix;
-      if (is_gt || (is_eq && e < need)) list[g + min(e, need)] = i0 + i;
-      g += is_gt;
-      e += is_eq;
+    for (int q = 0; q < kMine; ++q) mine += (key[q] > prefix ? 1u : 0u) + (key[q] == prefix ? 0x10000u : 0u);
+    uint32_t total;
+    const uint32_t before = block_scan(mine, sm.warp_sums, &total) - mine;
+    uint32_t g = gt_before + (before & 0xffffu), e = eq_before + (before >> 16);
+    if (mine) {
+#pragma unroll
+      for (int q = 0; q < kMine; ++q) {
+        const bool is_gt = key[q] > prefix, is_eq = key[q] == prefix;
+        if (is_gt || (is_eq && e < need)) list[g + min(e, need)] = i0 + q;
+        g += is_gt;
+        e += is_eq;
+      }
     }
     gt_before += total & 0xffffu;
     eq_before += total >> 16;
-  }
+  });
+}
+
+// `a.cluster` CTAs per (sequence, KV head), one cluster.
+__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_constant__ PagedEvict a) {
+  __shared__ SelectShared sm;
+  pdl_launch_dependents();
+  pdl_wait_primary();
+  const int C = a.cluster;
+  const int rank = int(blockIdx.x) % C, tid = threadIdx.x;
+  const int unit = int(blockIdx.x) / C;
+  const int n = max(0, min(a.kv.cap, a.kv.seq_lens[unit / a.kv.Hkv]));
+  const bool over = n > a.budget;
+  if (rank == 0 && tid == 0) a.state[unit] = make_int2(over ? 1 : 0, n);
+  if (!over) return;  // the whole cluster
+  int* list = a.list + size_t(unit) * a.budget;
+  const int m = n - a.recent, k = a.budget - a.recent;  // keep k of the first m, and the rest
+  for (int i = rank * kSelThreads + tid; i < a.recent; i += C * kSelThreads) list[k + i] = m + i;
+  if (k == 0) return;  // the whole cluster
+  const int per = ((m + C - 1) / C + 3) & ~3;
+  const int s0 = min(m, rank * per), s1 = min(m, s0 + per);
+  const float* w = a.weights + size_t(unit) * a.kv.cap;
+  if (per <= 4 * kSelThreads) select_tokens<4, true>(a, w, list, rank, s0, s1, k, sm);
+  else if (per <= kMost) select_tokens<16, true>(a, w, list, rank, s0, s1, k, sm);
+  else select_tokens<16, false>(a, w, list, rank, s0, s1, k, sm);
 }
 
 // ------------------------------------------------------------------ the move
 constexpr int kMoveThreads = 256;
-constexpr int kMoveVecs = 4;                                // 16-byte pieces per thread and chunk
+constexpr int kMoveVecs = 8;                                // 16-byte pieces per thread and chunk
 constexpr int kMoveStages = 3;                              // chunks in flight per CTA
 constexpr int kChunkVecs = kMoveThreads * kMoveVecs;
 
@@ -193,14 +310,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// Page of position p, or -1 (recorded) when the table names none of the pool's.
-__device__ __forceinline__ int page_at(const PagedEvict& a, const int* row, int p) {
-  const int id = row[a.kv.page_div.div(p)];
-  if (unsigned(id) < unsigned(a.kv.num_pages)) return id;
-  atomicCAS(a.status, kDevOk, kDevBadPage);
-  return -1;
-}
 
 // One column slice of one pool: v 16-byte pieces (a power of two) of every row.
 __device__ void move_rows(const PagedEvict& a, const int* list, const int* row, uint8_t* base, int64_t page_stride,
@@ -218,106 +327,158 @@ __device__ void move_rows(const PagedEvict& a, const int* list, const int* row, 
     if (still < kMoveThreads) break;
   }
   const uint32_t my = smem_u32(ring) + tid * 16;
-  auto at = [&](int p, int col) -> uint8_t* {
-    const int pg = page_at(a, row, p);
-    return pg < 0 ? nullptr : base + pg * page_stride + a.kv.page_div.mod(p) * tok_stride + 16 * col;
+  const int col = 16 * (tid & (v - 1));  // kMoveThreads is a multiple of v: the same piece of every row
+  const int row0 = tid >> shift, row_step = kMoveThreads >> shift;
+  // Two steps ahead of the fetch of a chunk its list entries are read, one step ahead its pages.
+  int idx[kMoveVecs], page[kMoveVecs], off[kMoveVecs];
+  auto read_list = [&](int c) {
+#pragma unroll
+    for (int i = 0; i < kMoveVecs; ++i) {
+      const int p = c * rows + row0 + i * row_step;
+      idx[i] = p < a.budget ? list[p] : -1;  // (past the last chunk too)
+    }
   };
-  unsigned got = 0;  // which pieces of the chunks in flight were fetched, 4 bits per stage
-  auto fetch = [&](int c) {
-    const int st = c % kMoveStages;
-    got &= ~(0xfu << (4 * st));
-    if (c < chunks) {
-      const uint8_t* src[kMoveVecs];
+  auto read_pages = [&]() {
 #pragma unroll
-      for (int i = 0; i < kMoveVecs; ++i) {
-        const int vec = tid + i * kMoveThreads;
-        const int p = c * rows + (vec >> shift);
-        src[i] = p < a.budget ? at(list[p], vec & (v - 1)) : nullptr;
+    for (int i = 0; i < kMoveVecs; ++i) {
+      page[i] = idx[i] < 0 ? 0 : row[a.kv.page_div.div(idx[i])];
+      off[i] = idx[i] < 0 ? -1 : a.kv.page_div.mod(idx[i]);  // -1: no row
+    }
+  };
+  unsigned got = 0;  // which pieces of the chunks in flight were fetched, kMoveVecs bits per stage
+  static_assert(kMoveVecs * kMoveStages <= 32, "one bit per piece in flight");
+  auto fetch = [&](int st) {
+    got &= ~(((1u << kMoveVecs) - 1u) << (kMoveVecs * st));
+#pragma unroll
+    for (int i = 0; i < kMoveVecs; ++i) {
+      if (off[i] < 0) continue;
+      if (unsigned(page[i]) < unsigned(a.kv.num_pages)) {
+        cp_async16(my + (st * kChunkVecs + i * kMoveThreads) * 16, base + page[i] * page_stride + off[i] * tok_stride + col);
+        got |= 1u << (kMoveVecs * st + i);
+      } else {
+        atomicCAS(a.status, kDevOk, kDevBadPage);
       }
-#pragma unroll
-      for (int i = 0; i < kMoveVecs; ++i)
-        if (src[i]) {
-          cp_async16(my + (st * kChunkVecs + i * kMoveThreads) * 16, src[i]);
-          got |= 1u << (4 * st + i);
-        }
     }
     cp_async_commit();
   };
-  for (int c = first; c < first + kMoveStages - 1; ++c) fetch(c);
+  read_list(first);
+  read_pages();
+  read_list(first + 1);
+  for (int c = first; c < first + kMoveStages - 1; ++c) {
+    fetch(c % kMoveStages);
+    read_pages();
+    read_list(c + 2);
+  }
   for (int c = first; c < chunks; ++c) {
-    fetch(c + kMoveStages - 1);
+    int to_page[kMoveVecs];
+    const int p0 = c * rows + row0;
+#pragma unroll
+    for (int i = 0; i < kMoveVecs; ++i) {
+      const int p = p0 + i * row_step;
+      to_page[i] = p < a.budget ? row[a.kv.page_div.div(p)] : -1;
+    }
+    fetch((c + kMoveStages - 1) % kMoveStages);
+    read_pages();
+    read_list(c + kMoveStages + 1);
     cp_async_wait<kMoveStages - 1>();
     __syncthreads();  // the whole chunk (and all before it) is read: its destinations are free
     const int st = c % kMoveStages;
 #pragma unroll
     for (int i = 0; i < kMoveVecs; ++i) {
-      if (!(got >> (4 * st + i) & 1u)) continue;
-      const int vec = tid + i * kMoveThreads;
-      uint8_t* dst = at(c * rows + (vec >> shift), vec & (v - 1));
-      if (dst) *reinterpret_cast<uint4*>(dst) = ring[st * kChunkVecs + vec];
+      if (!(got >> (kMoveVecs * st + i) & 1u)) continue;
+      if (unsigned(to_page[i]) >= unsigned(a.kv.num_pages)) {
+        atomicCAS(a.status, kDevOk, kDevBadPage);
+        continue;
+      }
+      uint8_t* dst = base + to_page[i] * page_stride + a.kv.page_div.mod(p0 + i * row_step) * tok_stride + col;
+      *reinterpret_cast<uint4*>(dst) = ring[st * kChunkVecs + tid + i * kMoveThreads];
     }
   }
   cp_async_wait<0>();
 }
 
-// Scales, weights and the new length of one (sequence, KV head), in the same chunk order.
-__device__ void move_scalars(const PagedEvict& a, const int* list, const int* row, int unit, int2 state) {
-  const int tid = threadIdx.x, kh = unit % a.kv.Hkv;
+// Page of position p, or -1 (recorded) when the table names none of the pool's.
+__device__ __forceinline__ int page_at(const PagedEvict& a, const int* row, int p) {
+  const int id = row[a.kv.page_div.div(p)];
+  if (unsigned(id) < unsigned(a.kv.num_pages)) return id;
+  atomicCAS(a.status, kDevOk, kDevBadPage);
+  return -1;
+}
+
+// The scales and weights of one (sequence, KV head), by one CTA in list order: a step is read by all threads before
+// any of it is written, and lands below the next step's sources.
+__device__ void move_scalars(const PagedEvict& a, const int* list, int unit, int2 state) {
+  constexpr int kVals = 4;
+  const int n = state.y;
+  const int tid = threadIdx.x, b = unit / a.kv.Hkv, kh = unit - b * a.kv.Hkv;
+  const int* row = a.kv.table + int64_t(b) * a.kv.table_stride;
   const float* w = a.weights + size_t(unit) * a.kv.cap;
   float* wo = a.weights_out + size_t(unit) * a.kv.cap;
-  if (kh == 0 && tid == 0) a.lens_out[unit / a.kv.Hkv] = state.x ? a.budget : state.y;
   if (!state.x) {
     if (wo != w)
-      for (int i = tid; i < state.y; i += kMoveThreads) wo[i] = w[i];
+      for (int i = tid; i < n; i += kMoveThreads) wo[i] = w[i];
     return;
   }
-  for (int p0 = 0; p0 < a.budget; p0 += kMoveThreads) {
-    const int p = p0 + tid;
-    const bool on = p < a.budget;
-    float x = 0.f;
-    __half ks = __half(0.f), vs = __half(0.f);
-    bool sc = false;
-    if (on) {
-      const int s = list[p];
-      x = w[s];
-      if (a.kv.int8) {
-        const int pg = page_at(a, row, s);
+  for (int p0 = 0; p0 < a.budget; p0 += kVals * kMoveThreads) {
+    int from[kVals];
+    float x[kVals];
+    __half ks[kVals], vs[kVals];
+#pragma unroll
+    for (int i = 0; i < kVals; ++i) {
+      const int p = p0 + i * kMoveThreads + tid;
+      from[i] = p < a.budget ? list[p] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kVals; ++i) x[i] = from[i] >= 0 ? w[from[i]] : 0.f;
+    if (a.kv.int8) {
+#pragma unroll
+      for (int i = 0; i < kVals; ++i) {
+        const int pg = from[i] >= 0 ? page_at(a, row, from[i]) : -1;
         if (pg >= 0) {
-          ks = a.kv.ks[pg * a.kv.ks_page + kh * a.kv.ks_head + a.kv.page_div.mod(s)];
-          vs = a.kv.vs[pg * a.kv.vs_page + kh * a.kv.vs_head + a.kv.page_div.mod(s)];
-          sc = true;
+          ks[i] = a.kv.ks[pg * a.kv.ks_page + kh * a.kv.ks_head + a.kv.page_div.mod(from[i])];
+          vs[i] = a.kv.vs[pg * a.kv.vs_page + kh * a.kv.vs_head + a.kv.page_div.mod(from[i])];
+        } else {
+          from[i] = -1;  // no scales
         }
       }
     }
     __syncthreads();
-    if (on) {
-      wo[p] = x;
-      const int pg = sc ? page_at(a, row, p) : -1;
+#pragma unroll
+    for (int i = 0; i < kVals; ++i) {
+      const int p = p0 + i * kMoveThreads + tid;
+      if (p >= a.budget) continue;
+      wo[p] = x[i];
+      const int pg = a.kv.int8 && from[i] >= 0 ? page_at(a, row, p) : -1;
       if (pg >= 0) {
-        a.kv.ks[pg * a.kv.ks_page + kh * a.kv.ks_head + a.kv.page_div.mod(p)] = ks;
-        a.kv.vs[pg * a.kv.vs_page + kh * a.kv.vs_head + a.kv.page_div.mod(p)] = vs;
+        a.kv.ks[pg * a.kv.ks_page + kh * a.kv.ks_head + a.kv.page_div.mod(p)] = ks[i];
+        a.kv.vs[pg * a.kv.vs_page + kh * a.kv.vs_head + a.kv.page_div.mod(p)] = vs[i];
       }
     }
   }
-  __syncthreads();  // in place: the last chunk's sources may lie behind the budget
-  for (int p = a.budget + tid; p < state.y; p += kMoveThreads) wo[p] = 0.f;
+  __syncthreads();  // in place: the last step's sources may lie behind the budget
+  for (int p = a.budget + tid; p < n; p += kMoveThreads) wo[p] = 0.f;
 }
 
-// Grid: (2 * slices + 1, B * Hkv).
+// Blocks: 2 * slices per (sequence, KV head) for the rows, then one each for the rest, which fills the last wave.
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ PagedEvict a) {
   extern __shared__ uint4 ring[];
   pdl_launch_dependents();
   pdl_wait_primary();
-  const int unit = int(blockIdx.y), job = int(blockIdx.x);
+  const int jobs = 2 * a.slices, units = a.kv.B * a.kv.Hkv;
+  const bool rest = int(blockIdx.x) >= units * jobs;
+  const int unit = rest ? int(blockIdx.x) - units * jobs : int(blockIdx.x) / jobs;
   const int2 state = a.state[unit];
   const int* list = a.list + size_t(unit) * a.budget;
   const int b = unit / a.kv.Hkv, kh = unit - b * a.kv.Hkv;
-  const int* row = a.kv.table + int64_t(b) * a.kv.table_stride;
-  if (job == 2 * a.slices) {
-    move_scalars(a, list, row, unit, state);
+  if (rest) {
+    // (here, not in the selection: lens_out may be the lengths that its CTAs read)
+    if (kh == 0 && threadIdx.x == 0) a.lens_out[b] = state.x ? a.budget : state.y;
+    move_scalars(a, list, unit, state);
     return;
   }
   if (!state.x) return;
+  const int* row = a.kv.table + int64_t(b) * a.kv.table_stride;
+  const int job = int(blockIdx.x) - unit * jobs;
   const bool is_v = job >= a.slices;
   const int elt = a.kv.int8 ? 1 : 2;
   const int width = a.kv.D * elt / a.slices;  // bytes
@@ -335,8 +496,19 @@ cudaError_t evict_prepare() {
   return cudaFuncSetAttribute(evict_move_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kMoveSmem));
 }
 
-cudaError_t launch_evict_paged(const PagedEvict& a, cudaStream_t stream) {
+cudaError_t launch_evict_paged(const PagedEvict& args, cudaStream_t stream) {
+  PagedEvict a = args;
   const int units = a.kv.B * a.kv.Hkv;
+  // The move: column slices until about 1000 CTAs exist, none narrower than a 32-byte sector.  16 sequences of
+  // 0 to 16K tokens -> 4096, 8 KV heads, D = 128: 2 slices 123 us, 4 slices 111 us, 8 slices 134 us (pieces of
+  // one 64-byte DRAM access fetched at different times).
+  a.slices = 1;
+  while (units * 2 * a.slices < 1024 && a.kv.D * (a.kv.int8 ? 1 : 2) / a.slices > 32) a.slices *= 2;
+  // The selection: one CTA while a full sequence is about what it holds in registers (one step and a half, so that a
+  // table with room to spare for 16K tokens does not pay a cluster's barriers: 31 us instead of 35 us for one such
+  // sequence of 8 KV heads), then clusters of 2, 4 and 8.
+  a.cluster = 1;
+  while (a.cluster < 8 && int64_t(a.cluster) * (kMost + kMost / 2) < a.kv.cap) a.cluster *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(units) * unsigned(a.cluster));
   cfg.blockDim = dim3(kSelThreads);
@@ -352,7 +524,7 @@ cudaError_t launch_evict_paged(const PagedEvict& a, cudaStream_t stream) {
   cfg.numAttrs = 2;
   cudaError_t e = cudaLaunchKernelEx(&cfg, evict_select_kernel, a);
   if (e != cudaSuccess) return e;
-  return launch_pdl(evict_move_kernel, dim3(2 * a.slices + 1, units), dim3(kMoveThreads), kMoveSmem, stream, a);
+  return launch_pdl(evict_move_kernel, dim3((2 * a.slices + 1) * units), dim3(kMoveThreads), kMoveSmem, stream, a);
 }
 
 }  // namespace fqkv

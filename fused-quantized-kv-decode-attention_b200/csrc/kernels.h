@@ -271,8 +271,7 @@ struct PagedEvict {
   int2* state;             // [B * Hkv]: over budget?, length (workspace)
   int* list;               // [B * Hkv][budget]: kept tokens in order (workspace)
   int budget, recent;
-  int cluster;             // selection CTAs per (sequence, KV head)
-  int slices;              // column slices of a row in the move
+  int cluster, slices;     // chosen by the launch: selection CTAs per (sequence, KV head); column slices of a row
   int* status;
 };
 cudaError_t evict_prepare();
