@@ -98,6 +98,7 @@ void init_device(DeviceState& ds, int dev) {
   if (e == cudaSuccess) e = fqkv::quantize_kernel_prepare(&ds.occ_quantize);
   for (int q = 0; q < 2 && e == cudaSuccess; ++q)
     for (int i = 0; i < 2 && e == cudaSuccess; ++i) e = fqkv::paged_attn_prepare(q == 1, i ? 128 : 64, ds.occ_paged[q][i]);
+  if (e == cudaSuccess) e = fqkv::append_paged_prepare();
   if (e == cudaSuccess) e = fqkv::evict_prepare();
   if (e != cudaSuccess) return bad(FQKV_ERR_CUDA, cudaGetErrorString(e));
 }
@@ -1131,7 +1132,10 @@ int fqkv_rope_append_paged(const fqkv_paged_kv_t* kv, int32_t model_dtype, const
   a.slots = reinterpret_cast<const int*>(slots);
   a.q_out = static_cast<__half*>(q_out);
   a.T = T; a.Hq = int(Hq);
+  a.sms = ds->sm_count;
   a.status = ds->status;
+  a.timeout_ns = g_timeout_ns.load();
+  a.debug_skip_loads = g_debug_skip_loads.load();
   cudaError_t e = fqkv::launch_append_paged(a, model_dtype == 1, reinterpret_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "paged append launch");
   return FQKV_OK;

@@ -258,8 +258,12 @@ struct PagedAppend {
   __half* q_out;           // [T, Hq, D]
   int64_t T;
   int Hq, axes;
+  int sms;
   int* status;
+  unsigned long long timeout_ns;
+  int debug_skip_loads;
 };
+cudaError_t append_paged_prepare();
 cudaError_t launch_append_paged(const PagedAppend& a, bool bf16, cudaStream_t stream);
 
 // One call of the eviction (evict_paged.cu).

@@ -106,8 +106,14 @@ class _DeviceGuard:
         return False
 
 
+# The current stream's handle without building a torch.cuda.Stream object (2.3 us of a decode call's host time).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    if _raw_stream is None or dev.index is None:
+        return torch.cuda.current_stream(dev).cuda_stream
+    return _raw_stream(dev.index)
 
 
 def workspace_bytes(kv_format: str, B: int, Hq: int, Hkv: int, N: int, D: int) -> int:
@@ -777,21 +783,28 @@ def quant_int4_per_token(X: torch.Tensor):
 
 # ------------------------------------------------------------------ paged KV cache
 def _index_tensor(op: str, name: str, t: torch.Tensor, dev: torch.device) -> None:
-    if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != torch.int32:
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.device != dev:
         _fail(op, name, f"{name} must be an int32 tensor on the inputs' device")
+
+
+def _index_vector(op: str, name: str, t: torch.Tensor, n: int, dev: torch.device) -> None:
+    _index_tensor(op, name, t, dev)
+    if t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+        _fail(op, name, f"{name} must be a contiguous int32 tensor of {n} (got {tuple(t.shape)})")
 
 
 def _paged_kv(op: str, K, V, Ks, Vs, block_table, seq_lens, dev: torch.device):
     """Checks a paged cache; returns (packed descriptor, B, Hkv, D, tokens a sequence can hold, int8)."""
-    if K.dim() != 4 or V.shape != K.shape:
+    shape = K.shape
+    if len(shape) != 4 or V.shape != shape:
         _fail(op, "shape", "K and V must both be [num_pages, Hkv, page_size, D]")
     int8 = Ks is not None or Vs is not None
-    key, code = ("int8", torch.int8) if int8 else ("fp16", torch.float16)
-    if K.dtype != code or V.dtype != code:
-        _fail(op, key, f"K and V must be {code} (got {K.dtype}, {V.dtype})")
-    P, Hkv, page, D = K.shape
+    code = torch.int8 if int8 else torch.float16
+    if K.dtype is not code or V.dtype is not code:
+        _fail(op, "int8" if int8 else "fp16", f"K and V must be {code} (got {K.dtype}, {V.dtype})")
+    P, Hkv, page, D = shape
     sk, sv = K.stride(), V.stride()
-    if D not in (64, 128):
+    if D != 64 and D != 128:
         _fail(op, "D", f"head_dim must be 64 or 128 (got {D})")
     if sk[3] != 1 or sv[3] != 1:
         _fail(op, "stride", "K and V must be contiguous over D")
@@ -799,23 +812,25 @@ def _paged_kv(op: str, K, V, Ks, Vs, block_table, seq_lens, dev: torch.device):
     if block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
         _fail(op, "block_table", "block_table must be [B, max_pages] with contiguous rows")
     B, max_pages = block_table.shape
+    lens = 0
     if seq_lens is not None:
-        _index_tensor(op, "seq_lens", seq_lens, dev)
-        if seq_lens.shape != (B,) or (B > 1 and seq_lens.stride(0) != 1):
-            _fail(op, "seq_lens", f"seq_lens must be contiguous [B = {B}]")
+        _index_vector(op, "seq_lens", seq_lens, B, dev)
+        lens = seq_lens.data_ptr()
+    ks = vs = 0
     sks = svs = (0, 0)
     if int8:
         _require_cuda(op, K, Ks, Vs)
         _require_dtype(op, "fp16", torch.float16, Ks=Ks, Vs=Vs)
-        _require_shape(op, "Ks", Ks, (P, Hkv, page))
-        _require_shape(op, "Vs", Vs, (P, Hkv, page))
-        if Ks.stride(2) != 1 or Vs.stride(2) != 1:
+        if Ks.shape != shape[:3] or Vs.shape != shape[:3]:
+            _fail(op, "shape", f"Ks and Vs must be [num_pages, Hkv, page_size] = {tuple(shape[:3])}")
+        sks, svs = Ks.stride(), Vs.stride()
+        if sks[2] != 1 or svs[2] != 1:
             _fail(op, "stride", "Ks and Vs must be contiguous over a page's tokens")
-        sks, svs = Ks.stride()[:2], Vs.stride()[:2]
+        ks, vs = Ks.data_ptr(), Vs.data_ptr()
     desc = _native.PAGED_KV.pack(
-        _native.KV_INT8 if int8 else _native.KV_F16, 0, page, P, max_pages, B, Hkv, D, K.data_ptr(), V.data_ptr(),
-        Ks.data_ptr() if int8 else 0, Vs.data_ptr() if int8 else 0, sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], *sks, *svs,
-        block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr() if seq_lens is not None else 0)
+        _native.KV_INT8 if int8 else _native.KV_F16, 0, page, P, max_pages, B, Hkv, D, K.data_ptr(), V.data_ptr(), ks, vs,
+        sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], sks[0], sks[1], svs[0], svs[1], block_table.data_ptr(),
+        block_table.stride(0), lens)
     return desc, B, Hkv, D, max_pages * page, int8
 
 
@@ -859,7 +874,7 @@ def _decode_paged(op, q, K, V, Ks, Vs, block_table, seq_lens, out, workspace, we
         _fail(op, "shape", f"q has shape {tuple(q.shape)}, expected ({B}, Hq, {D})")
     if weights is not None:
         _slot_weights(op, "weights", weights, (B, Hkv, cap), dev)
-    out = _kv_out(op, q, out, q.shape, dev)
+    out = torch.empty_like(q) if out is None else _kv_out(op, q, out, q.shape, dev)
     lib = _native.lib()
     with _DeviceGuard(dev):
         need = 0
@@ -869,7 +884,8 @@ def _decode_paged(op, q, K, V, Ks, Vs, block_table, seq_lens, out, workspace, we
         ws, nb, keep = _scratch(op, workspace, need, dev)
         rc = lib.fqkv_decode_attn_paged(desc, 1 if out.dtype == torch.bfloat16 else 0, q.data_ptr(), out.data_ptr(), Hq,
                                         None if weights is None else weights.data_ptr(), ws, nb, _stream(dev))
-    _native.check(rc, f"launch: {op}")
+    if rc:
+        _native.check(rc, f"launch: {op}")
     return out
 
 
@@ -947,32 +963,26 @@ def rope_qkv_append_paged(qkv: torch.Tensor, cos_table: torch.Tensor, sin_table:
     if q_out.shape[2] != D or qkv.shape[0] != T or qkv.shape[1] < (Hq + 2 * Hkv) * D:
         _fail(op, "shape", f"qkv must be [T, >= (Hq + 2 Hkv) D] and q_out [T, Hq, {D}] "
                            f"(got {tuple(qkv.shape)}, {tuple(q_out.shape)})")
-    for name, t in (("cos_table", cos_table), ("sin_table", sin_table)):
-        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != D // 2 or t.shape != cos_table.shape \
-                or not t.is_contiguous():
-            _fail(op, "tables", f"{name} must be contiguous float32 [rows, D/2 = {D // 2}]")
-    _index_tensor(op, "slots", slots, dev)
+    rows = cos_table.shape[0] if cos_table.dim() else 0
+    if cos_table.shape != (rows, D // 2) or sin_table.shape != (rows, D // 2) or cos_table.dtype is not torch.float32 \
+            or sin_table.dtype is not torch.float32 or not cos_table.is_contiguous() or not sin_table.is_contiguous():
+        _fail(op, "tables", f"cos_table and sin_table must be contiguous float32 [rows, D/2 = {D // 2}]")
+    _index_vector(op, "slots", slots, T, dev)
     _index_tensor(op, "positions", positions, dev)
-    if slots.shape != (T,) or (T > 1 and slots.stride(0) != 1):
-        _fail(op, "slots", f"slots must be contiguous [T = {T}]")
     if positions.dim() not in (1, 2) or positions.shape[-1] != T or (T > 1 and positions.stride(-1) != 1):
         _fail(op, "positions", f"positions must be [T = {T}] or [A, T] with contiguous rows")
     A = positions.shape[0] if positions.dim() == 2 else 1
     if A > 1:
         if axes is None:
             _fail(op, "axes", "several position axes need axes [D/2]")
-        _index_tensor(op, "axes", axes, dev)
-        if axes.shape != (D // 2,) or not axes.is_contiguous():
-            _fail(op, "axes", f"axes must be contiguous int32 [D/2 = {D // 2}]")
+        _index_vector(op, "axes", axes, D // 2, dev)
     if seq_ids is not None:
-        _index_tensor(op, "seq_ids", seq_ids, dev)
-        if seq_ids.shape != (T,) or (T > 1 and seq_ids.stride(0) != 1):
-            _fail(op, "seq_ids", f"seq_ids must be contiguous [T = {T}]")
+        _index_vector(op, "seq_ids", seq_ids, T, dev)
     with _DeviceGuard(dev):
         rc = _native.lib().fqkv_rope_append_paged(
             desc, 1 if qkv.dtype == torch.bfloat16 else 0, qkv.data_ptr(),
             qkv.stride(0) if T > 1 else (Hq + 2 * Hkv) * D, cos_table.data_ptr(),
-            sin_table.data_ptr(), cos_table.shape[0], positions.data_ptr(), positions.stride(0) if A > 1 else T, A,
+            sin_table.data_ptr(), rows, positions.data_ptr(), positions.stride(0) if A > 1 else T, A,
             axes.data_ptr() if A > 1 else None, None if seq_ids is None else seq_ids.data_ptr(), slots.data_ptr(),
             q_out.data_ptr(), T, Hq, _stream(dev))
     _native.check(rc, f"launch: {op}")
@@ -1003,9 +1013,7 @@ def evict_kvcache_paged(K: torch.Tensor, V: torch.Tensor, block_table: torch.Ten
     if lens_out is None:
         lens_out = torch.empty_like(seq_lens)
     else:
-        _index_tensor(op, "lens_out", lens_out, dev)
-        if lens_out.shape != (B,) or (B > 1 and lens_out.stride(0) != 1):
-            _fail(op, "lens_out", f"lens_out must be contiguous [B = {B}]")
+        _index_vector(op, "lens_out", lens_out, B, dev)
     lib = _native.lib()
     with _DeviceGuard(dev):
         need = 0

@@ -391,10 +391,9 @@ size_t fqkv_paged_workspace_bytes(int kv_format, int64_t B, int64_t Hq, int64_t 
  * slots[t] of sequence seq_ids[t] (NULL: sequence t), as f16, or as the codes and scale
  * that fqkv_quantize_int8_per_token gives for the f16 row.  All arithmetic is
  * fp32, rounded once to f16.  A token with a negative slot is padding:
- * nothing of it is written, q_out included.  One whose sequence, slot or
- * position is out of range is not written either and records status 66 (65: its page), an
- * axis out of range records 66 and its pairs are undefined.  Two tokens of one
- * call must not share a slot.  seq_lens is not used.  Extends
+ * nothing of it is written, q_out included.  One whose sequence, slot, axes or
+ * positions are out of range is not written either and records status 66 (65:
+ * its page).  Two tokens of one call must not share a slot.  seq_lens is not used.  Extends
  * fqkv_rope_qkv_append, whose rounding follows transformers' in the model dtype. */
 int fqkv_rope_append_paged(const fqkv_paged_kv_t* kv, int32_t model_dtype, const void* qkv, int64_t qkv_row_stride,
                            const float* cos_table, const float* sin_table, int64_t table_rows, const int32_t* positions,

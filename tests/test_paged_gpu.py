@@ -398,11 +398,11 @@ def _check_append(fqkv, c, before, qkv, cos, sin, pos, axes, slots, seqs, q_out,
 @pytest.mark.parametrize("model", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("D,Hq,Hkv,axes,interleaved", [(64, 8, 2, 1, False), (128, 7, 7, 3, False), (64, 3, 1, 3, True),
                                                         (128, 33, 11, 2, True), (128, 1, 1, 1, False)])
-@pytest.mark.parametrize("tokens", ["decode", "packed", "many"])
+@pytest.mark.parametrize("tokens", ["decode", "packed", "many", "prefill"])
 def test_append(fqkv, model, D, Hq, Hkv, axes, interleaved, tokens):
     g = torch.Generator().manual_seed(D + Hq)
-    lens = [5, 0, 31, 16] if tokens != "many" else [0, 0]
-    room = 1 if tokens == "decode" else (17 if tokens == "packed" else 300)
+    lens = [5, 0, 31, 16] if tokens in ("decode", "packed") else [0, 0]
+    room = {"decode": 1, "packed": 17, "many": 300, "prefill": 900}[tokens]  # prefill: more than 1000 tokens, the other kernel
     cos, sin = _tables(500, D)
     sec = {1: [D // 2], 2: [D // 2 - 9, 9], 3: [D // 2 - 2 * (D // 8), D // 8, D // 8]}[axes]
     amap = fqkv.rope_axes(sec, interleaved)
@@ -500,6 +500,61 @@ def test_append_out_of_range_token_is_reported_and_not_written(fqkv, what):
         assert (q_out[1] == 5).all() and not (q_out[0] == 5).all() and not (q_out[2] == 5).all()
         rows = c.V.abs().sum((1, 3)) > 0
         assert int(rows.sum()) == 2
+    _clean(fqkv)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_append_prefill_with_bad_tokens_and_padding(fqkv, int8):
+    """Among 1500 tokens some are padding and one of each kind is out of range: only those are left out."""
+    D, Hq, Hkv, T = 128, 4, 2, 1500
+    c = Cache(fqkv, [0, 0], Hkv, D, 32, int8, room=800)
+    c.K, c.V = torch.zeros_like(c.K), torch.zeros_like(c.V)
+    cos, sin = _tables(64, D)
+    i = torch.arange(T, dtype=torch.int32)
+    slots, seqs, pos = i % 750, i // 750, torch.stack([i % 64, i % 63, i % 62])
+    c.table[1, 9] = c.P + 5                        # slots 288 .. 319 of sequence 1: tokens 1038 .. 1069
+    slots[7], seqs[8], pos[1, 9], slots[10] = c.cap, 2, 64, -1
+    bad = [7, 8, 9, 10] + list(range(1038, 1070))
+    qkv = (torch.rand(T, (Hq + 2 * Hkv) * D, generator=torch.Generator().manual_seed(1)) + 0.5).bfloat16().cuda()
+    q_out = torch.full((T, Hq, D), 5.0, dtype=torch.float16, device="cuda")
+    fqkv.rope_qkv_append_paged(qkv, cos, sin, pos.contiguous().cuda(), slots.cuda(), c.table, q_out, c.K, c.V, c.Ks, c.Vs,
+                               axes=fqkv.rope_axes([16, 24, 24]), seq_ids=seqs.cuda())
+    with pytest.raises(RuntimeError, match="page outside|out of range"):
+        fqkv.ops.check_device_status(torch.device("cuda", 0), "append")
+    left = (q_out == 5).flatten(1).all(1).cpu()
+    assert left.nonzero().flatten().tolist() == bad
+    written = (c.V != 0).flatten(3).any(3).any(1)   # v is never 0 here
+    want = torch.zeros_like(written)
+    for t in range(T):
+        if t not in bad:
+            want[int(c.table[int(seqs[t]), int(slots[t]) // 32]), int(slots[t]) % 32] = True
+    assert torch.equal(written, want)
+    _clean(fqkv)
+
+
+def test_append_stalled_pipeline_gives_up(fqkv):
+    """Rows that never arrive: the prefill kernel's waits end with status 61 and the context stays usable."""
+    lib = fqkv.native.lib()
+    D, Hq, Hkv, T = 64, 4, 2, 1200
+    c = Cache(fqkv, [0, 0], Hkv, D, 16, False, room=600)
+    cos, sin = _tables(600, D)
+    i = torch.arange(T, dtype=torch.int32).cuda()
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * D, generator=torch.Generator().manual_seed(1)).half().cuda()
+    q_out = torch.zeros(T, Hq, D, dtype=torch.float16, device="cuda")
+    call = lambda: fqkv.rope_qkv_append_paged(qkv, cos, sin, i % 600, i % 600, c.table, q_out, c.K, c.V,  # noqa: E731
+                                              seq_ids=i // 600)
+    lib.fqkv_set_wait_timeout_ms(50)
+    lib.fqkv_debug_skip_loads(1)
+    try:
+        call()
+        torch.cuda.synchronize()
+    finally:
+        lib.fqkv_debug_skip_loads(0)
+        lib.fqkv_set_wait_timeout_ms(2000)
+    assert fqkv.ops.device_status(torch.device("cuda", 0)) == 61
+    call()
+    torch.cuda.synchronize()
+    assert bool((q_out != 0).flatten(1).any(1).all())
     _clean(fqkv)
 
 
