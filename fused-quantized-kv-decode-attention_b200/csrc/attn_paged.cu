@@ -22,8 +22,15 @@
 //    the score accumulators hold them and 8 heads fill all 8 columns: half the MMAs and half the accumulator
 //    registers of the P V order, which leaves half of its 16 rows empty.  More than 8 heads take two column
 //    tiles, so up to 16 heads share one pass over K and V.
-//  * int8: a code becomes the exact fp16 number by one byte permute into 1024 + (code + 128) and one
-//    subtraction.  The K scale multiplies the score.  The V scale multiplies the probability before it is
+//  * int8, S: integer MMAs (m16n8k32) on the codes as they lie in memory.  A head's q is a fixed-point number of
+//    22 bits, q 2^k = hi 65536 + mid 256 + lo with max |q| 2^k in [2^21, 2^22): an fp16 q is exact in it down to 2^-11 of
+//    the largest, so the sums of products are exact integers and the score is rounded only when the three are put
+//    together.  Up to 8 heads: rows 0-7 of one MMA are hi, rows 8-15 mid, a second one takes lo.  Against codes
+//    converted to fp16 this saves 80 of about 290 instructions per warp and 16 keys at D = 128.
+//  * int8, P V: a code becomes the fp16 number 1152 + code by one byte permute (of code + 128), and a second MMA with
+//    a constant tile takes 1152 P away again, 16 keys at a time: the subtraction costs tensor-core time, which is
+//    there, and no instruction per code; what it rounds is 2^-24 of 1152 P, 7e-5 of a code's step.  The K scale multiplies
+//    the score.  The V scale multiplies the probability before it is
 //    rounded to fp16, times a power of two that puts the unit's largest V scale so far in [2^13, 2^14): small
 //    scales keep all their bits, and the factor leaves exactly at the end of the unit.
 //  * Scores, maxima, sums and outputs are fp32; the probabilities are rounded to fp16 once, as the operand of
@@ -198,13 +205,37 @@ __device__ __forceinline__ void store_out(const PagedLaunch& a, size_t idx, floa
   else static_cast<__half*>(a.out)[idx] = __float2half_rn(v);
 }
 
-// Two halves 1024 + u, 1024 + v of two bytes u, v of x (code + 128) minus 1152: the codes, exactly.
+// Two bytes of x (code + 128) as the fp16 numbers 1152 + code.
 template <uint32_t kSel>
 __device__ __forceinline__ uint32_t codes_to_half2(uint32_t x) {
   uint32_t h;
   asm("prmt.b32 %0, %1, %2, %3;" : "=r"(h) : "r"(x), "r"(0x64646464u), "n"(kSel));
-  const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&h), __half2half2(__ushort_as_half(0x6480u)));
-  return *reinterpret_cast<const uint32_t*>(&r);
+  return h;
+}
+constexpr uint32_t kMinus1152 = 0xE480E480u;  // two fp16 -1152
+
+// D(16x8, s32) += A(16x32, s8, row) * B(32x8, s8, col).
+__device__ __forceinline__ void mma_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Four q values times the power of two f as three planes of signed bytes: v = hi 65536 + mid 256 + lo, |v| < 2^22.
+__device__ __forceinline__ void q_planes(const uint2& q, float f, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&q.x));
+  const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&q.y));
+  const int v[4] = {__float2int_rn(x.x * f), __float2int_rn(x.y * f), __float2int_rn(y.x * f), __float2int_rn(y.y * f)};
+  hi = mid = lo = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int l = int(int8_t(v[i] & 0xff)), v1 = (v[i] - l) >> 8;
+    const int m = int(int8_t(v1 & 0xff)), h = (v1 - m) >> 8;
+    lo |= uint32_t(l & 0xff) << (8 * i);
+    mid |= uint32_t(m & 0xff) << (8 * i);
+    hi |= uint32_t(h & 0xff) << (8 * i);
+  }
 }
 
 // kNT: column tiles of 8 heads (1: up to 8 heads per unit, 2: up to 16).
@@ -343,23 +374,60 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
     const int gvalid = min(a.GP, a.G - p.grp * a.GP);
     const size_t row_base = size_t(p.b) * a.Hq + h0;
 
-    // Q fragments.  fp16: k = 2t, 2t + 1 and 2t + 8, 2t + 9 of each 16 dimensions; int8: the four
-    // consecutive dimensions 4t .. 4t + 3 in their place, as the lane finds them in a row of codes.
-    uint32_t qa[D / 16][2 * kNT];
+    // Q fragments.  fp16: k = 2t, 2t + 1 and 2t + 8, 2t + 9 of every 16 dimensions.  int8: the planes of dimensions
+    // 4t .. 4t + 3 and 16 + 4t .. of every 32.
+    constexpr int kQ = kI8 ? (kNT == 1 ? 6 : 12) : 2 * kNT, kQS = kI8 ? D / 32 : D / 16;
+    uint32_t qa[kQS][kQ];
+    float q_scale[kNT];  // int8: softmax scale over the head's fixed-point unit
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
       const bool on = g + 8 * nt < gvalid;
       const __half* qrow = static_cast<const __half*>(a.q) + (row_base + g + 8 * nt) * D;
+      if constexpr (!kI8) {
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        uint2 v = make_uint2(0u, 0u);
-        if (on) {
-          const int o0 = 16 * kk + (kI8 ? 4 * t4 : 2 * t4);
-          v.x = *reinterpret_cast<const uint32_t*>(qrow + o0);
-          v.y = *reinterpret_cast<const uint32_t*>(qrow + o0 + (kI8 ? 2 : 8));
+        for (int kk = 0; kk < kQS; ++kk) {
+          qa[kk][2 * nt] = on ? *reinterpret_cast<const uint32_t*>(qrow + 16 * kk + 2 * t4) : 0u;
+          qa[kk][2 * nt + 1] = on ? *reinterpret_cast<const uint32_t*>(qrow + 16 * kk + 2 * t4 + 8) : 0u;
         }
-        qa[kk][2 * nt] = v.x;
-        qa[kk][2 * nt + 1] = v.y;
+      } else {
+        uint2 raw[2 * kQS];
+        uint32_t top = 0;  // largest magnitude, as bits: inf and NaN stand above all numbers
+#pragma unroll
+        for (int i = 0; i < 2 * kQS; ++i) {
+          raw[i] = make_uint2(0u, 0u);
+          if (on) {  // q is 4-byte aligned
+            raw[i].x = *reinterpret_cast<const uint32_t*>(qrow + 16 * i + 4 * t4);
+            raw[i].y = *reinterpret_cast<const uint32_t*>(qrow + 16 * i + 4 * t4 + 2);
+          }
+          top = max(top, max(max(raw[i].x & 0x7fffu, (raw[i].x >> 16) & 0x7fffu), max(raw[i].y & 0x7fffu, (raw[i].y >> 16) & 0x7fffu)));
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^k = 2^(21 - floor(log2 max |q|)), by the exponent field
+        const int e = top == 0u ? 127 : (__float_as_int(__half2float(__ushort_as_half(uint16_t(top)))) >> 23);
+        const float unit = __int_as_float((127 + 21 + 127 - e) << 23);
+        q_scale[nt] = top >= 0x7c00u ? __int_as_float(0x7fc00000) : a.sm_scale_log2 / unit;
+#pragma unroll
+        for (int kk = 0; kk < kQS; ++kk) {
+          uint32_t hi[2], mid[2], lo[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) q_planes(raw[2 * kk + i], unit, hi[i], mid[i], lo[i]);
+          if constexpr (kNT == 1) {
+            qa[kk][0] = hi[0];
+            qa[kk][1] = mid[0];
+            qa[kk][2] = hi[1];
+            qa[kk][3] = mid[1];
+            qa[kk][4] = lo[0];
+            qa[kk][5] = lo[1];
+          } else {
+            qa[kk][nt] = hi[0];
+            qa[kk][2 + nt] = hi[1];
+            qa[kk][4 + nt] = mid[0];
+            qa[kk][6 + nt] = mid[1];
+            qa[kk][8 + nt] = lo[0];
+            qa[kk][10 + nt] = lo[1];
+          }
+        }
       }
     }
     float o[kNT][D / 16][4];
@@ -393,33 +461,52 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
         // ---- S = Q K^T
         float sc[NJ][4];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
-        auto mma_s = [&](float(&d)[4], int kk, uint32_t b0, uint32_t b1) {
-          if constexpr (kNT == 1) mma_16816(d, qa[kk][0], 0u, qa[kk][1], 0u, b0, b1);
-          else mma_16816(d, qa[kk][0], qa[kk][2], qa[kk][1], qa[kk][3], b0, b1);
-        };
-#pragma unroll
         for (int kb = 0; kb < C::KPW / 16; ++kb) {
           const uint32_t at = sk + k_off + uint32_t(16 * kb * C::RB);
           if constexpr (!kI8) {
 #pragma unroll
+            for (int j = 0; j < 2; ++j) sc[2 * kb + j][0] = sc[2 * kb + j][1] = sc[2 * kb + j][2] = sc[2 * kb + j][3] = 0.f;
+#pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
-              uint32_t b0, b1, b2, b3;
-              ldmatrix_x4(chunk_at<D, kI8>(at, kk), b0, b1, b2, b3);
-              mma_s(sc[2 * kb], kk, b0, b1);
-              mma_s(sc[2 * kb + 1], kk, b2, b3);
-            }
-          } else {
+              uint32_t b[4];
+              ldmatrix_x4(chunk_at<D, kI8>(at, kk), b[0], b[1], b[2], b[3]);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; kk += 2) {
-              uint32_t b[4];  // (keys 0-7, chunk kk), (keys 0-7, kk + 1), (keys 8-15, kk), (keys 8-15, kk + 1)
-              ldmatrix_x4(chunk_at<D, kI8>(at, kk / 2), b[0], b[1], b[2], b[3]);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t x = b[i] ^ 0x80808080u;
-                mma_s(sc[2 * kb + (i >> 1)], kk + (i & 1), codes_to_half2<0x4140>(x), codes_to_half2<0x4342>(x));
+              for (int j = 0; j < 2; ++j) {
+                if constexpr (kNT == 1) mma_16816(sc[2 * kb + j], qa[kk][0], 0u, qa[kk][1], 0u, b[2 * j], b[2 * j + 1]);
+                else mma_16816(sc[2 * kb + j], qa[kk][0], qa[kk][2], qa[kk][1], qa[kk][3], b[2 * j], b[2 * j + 1]);
               }
             }
+          } else {
+            constexpr int kAcc = kNT == 1 ? 2 : 3;
+            int acc[2][kAcc][4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int i = 0; i < kAcc; ++i) acc[j][i][0] = acc[j][i][1] = acc[j][i][2] = acc[j][i][3] = 0;
+#pragma unroll
+            for (int kk = 0; kk < D / 32; ++kk) {
+              uint32_t b[4];  // (keys 0-7, chunk 2 kk), (keys 0-7, 2 kk + 1), (keys 8-15, 2 kk), (keys 8-15, 2 kk + 1)
+              ldmatrix_x4(chunk_at<D, kI8>(at, kk), b[0], b[1], b[2], b[3]);
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                if constexpr (kNT == 1) {
+                  mma_16832(acc[j][0], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b[2 * j], b[2 * j + 1]);
+                  mma_16832(acc[j][1], qa[kk][4], 0u, qa[kk][5], 0u, b[2 * j], b[2 * j + 1]);
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 3; ++i)
+                    mma_16832(acc[j][i], qa[kk][4 * i], qa[kk][4 * i + 1], qa[kk][4 * i + 2], qa[kk][4 * i + 3], b[2 * j],
+                              b[2 * j + 1]);
+                }
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int e = 0; e < 2 * kNT; ++e) {
+                const int hi = acc[j][0][e], mid = kNT == 1 ? acc[j][0][2 + e] : acc[j][1][e], lo = acc[j][kAcc - 1][e];
+                sc[2 * kb + j][e] = fmaf(float(hi), 65536.f, fmaf(float(mid), 256.f, float(lo)));
+              }
           }
         }
         // ---- online softmax in the log2 domain; this lane: heads g (+ 8), keys k0 + r0 + 8j + 2 t4 + e
@@ -427,19 +514,18 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
           const int kq = r0 + 8 * j + 2 * t4;
-          float ks0 = a.sm_scale_log2, ks1 = a.sm_scale_log2;
+          float2 kf = make_float2(1.f, 1.f);
           if constexpr (kI8) {
-            const float2 kf = __half22float2(*reinterpret_cast<const __half2*>(scales + kq));
+            kf = __half22float2(*reinterpret_cast<const __half2*>(scales + kq));
             const float2 vf = __half22float2(*reinterpret_cast<const __half2*>(scales + C::TK + kq));
-            ks0 *= kf.x;
-            ks1 *= kf.y;
             vs[j][0] = (!kMask || k0 + kq < p.len) ? vf.x : 0.f;
             vs[j][1] = (!kMask || k0 + kq + 1 < p.len) ? vf.y : 0.f;
           }
 #pragma unroll
           for (int nt = 0; nt < kNT; ++nt) {
-            sc[j][2 * nt] = (!kMask || k0 + kq < p.len) ? sc[j][2 * nt] * ks0 : -INFINITY;
-            sc[j][2 * nt + 1] = (!kMask || k0 + kq + 1 < p.len) ? sc[j][2 * nt + 1] * ks1 : -INFINITY;
+            const float qs = kI8 ? q_scale[nt] : a.sm_scale_log2;
+            sc[j][2 * nt] = (!kMask || k0 + kq < p.len) ? sc[j][2 * nt] * (kI8 ? qs * kf.x : qs) : -INFINITY;
+            sc[j][2 * nt + 1] = (!kMask || k0 + kq + 1 < p.len) ? sc[j][2 * nt + 1] * (kI8 ? qs * kf.y : qs) : -INFINITY;
           }
           if (a.scores) {
 #pragma unroll
@@ -551,7 +637,10 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
                 const uint32_t lo0 = codes_to_half2<0x4240>(v[2 * i]), hi0 = codes_to_half2<0x4341>(v[2 * i]);
                 const uint32_t lo1 = codes_to_half2<0x4240>(v[2 * i + 1]), hi1 = codes_to_half2<0x4341>(v[2 * i + 1]);
 #pragma unroll
-                for (int nt = 0; nt < kNT; ++nt) mma_16816(o[nt][dd + i], lo0, hi0, lo1, hi1, pb[nt][0], pb[nt][1]);
+                for (int nt = 0; nt < kNT; ++nt) {
+                  mma_16816(o[nt][dd + i], lo0, hi0, lo1, hi1, pb[nt][0], pb[nt][1]);
+                  mma_16816(o[nt][dd + i], kMinus1152, kMinus1152, kMinus1152, kMinus1152, pb[nt][0], pb[nt][1]);
+                }
               }
             }
           }
