@@ -223,19 +223,19 @@ __device__ __forceinline__ void mma_16832(int (&d)[4], uint32_t a0, uint32_t a1,
 }
 
 // Four q values times the power of two f as three planes of signed bytes: v = hi 65536 + mid 256 + lo, |v| < 2^22.
+// x f + 2^23 + 2^22 has the integer v + 2^22 (rounded to nearest) in its mantissa; v + 0x808080 has the digits
+// plus 128 in its bytes.
 __device__ __forceinline__ void q_planes(const uint2& q, float f, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
   const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&q.x));
   const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&q.y));
-  const int v[4] = {__float2int_rn(x.x * f), __float2int_rn(x.y * f), __float2int_rn(y.x * f), __float2int_rn(y.y * f)};
-  hi = mid = lo = 0u;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int l = int(int8_t(v[i] & 0xff)), v1 = (v[i] - l) >> 8;
-    const int m = int(int8_t(v1 & 0xff)), h = (v1 - m) >> 8;
-    lo |= uint32_t(l & 0xff) << (8 * i);
-    mid |= uint32_t(m & 0xff) << (8 * i);
-    hi |= uint32_t(h & 0xff) << (8 * i);
-  }
+  auto digits = [&](float z) {
+    return uint32_t(__float_as_int(fmaf(z, f, 12582912.f))) + (0x808080u - 0x400000u);
+  };
+  const uint32_t u0 = digits(x.x), u1 = digits(x.y), u2 = digits(y.x), u3 = digits(y.y);
+  const uint32_t p01 = __byte_perm(u0, u1, 0x5140), p23 = __byte_perm(u2, u3, 0x5140);  // lo, lo, mid, mid
+  lo = __byte_perm(p01, p23, 0x5410) ^ 0x80808080u;
+  mid = __byte_perm(p01, p23, 0x7632) ^ 0x80808080u;
+  hi = __byte_perm(__byte_perm(u0, u1, 0x0062), __byte_perm(u2, u3, 0x0062), 0x5410) ^ 0x80808080u;
 }
 
 // kNT: column tiles of 8 heads (1: up to 8 heads per unit, 2: up to 16).
