@@ -782,74 +782,118 @@ def quant_int4_per_token(X: torch.Tensor):
 
 
 # ------------------------------------------------------------------ paged KV cache
-def _index_tensor(op: str, name: str, t: torch.Tensor, dev: torch.device) -> None:
-    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.device != dev:
-        _fail(op, name, f"{name} must be an int32 tensor on the inputs' device")
+# A decode step calls these every layer, so their checks are written for host time: device numbers instead of device
+# objects, no keyword dictionaries, messages built only when something is wrong.
+_I32, _F16, _F32, _BF16, _I8 = torch.int32, torch.float16, torch.float32, torch.bfloat16, torch.int8
 
 
-def _index_vector(op: str, name: str, t: torch.Tensor, n: int, dev: torch.device) -> None:
-    _index_tensor(op, name, t, dev)
-    if t.shape != (n,) or (n > 1 and t.stride(0) != 1):
-        _fail(op, name, f"{name} must be a contiguous int32 tensor of {n} (got {tuple(t.shape)})")
+def _gpu_of(op: str, *ts) -> int:
+    """The number of the GPU that holds all of ts."""
+    try:
+        idx = ts[0].get_device()
+        for t in ts:
+            if t.get_device() != idx:
+                _fail(op, "cuda", "all tensors must be on the same device")
+    except AttributeError:
+        _fail(op, "cuda", "all tensors must be CUDA tensors (there is no CPU path)")
+    if idx < 0:
+        _fail(op, "cuda", "all tensors must be CUDA tensors (there is no CPU path)")
+    return idx
 
 
-def _paged_kv(op: str, K, V, Ks, Vs, block_table, seq_lens, dev: torch.device):
-    """Checks a paged cache; returns (packed descriptor, B, Hkv, D, tokens a sequence can hold, int8)."""
+def _on_gpu(idx: int, fn, *args):
+    """fn(*args) with GPU idx current."""
+    if torch.cuda.current_device() == idx:
+        return fn(*args)
+    with torch.cuda.device(idx):
+        return fn(*args)
+
+
+def _stream_of(idx: int) -> int:
+    return _raw_stream(idx) if _raw_stream is not None else torch.cuda.current_stream(idx).cuda_stream
+
+
+def _index_vector(op: str, name: str, t: torch.Tensor, n: int) -> None:
+    if t.dtype is not _I32 or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+        _fail(op, name, f"{name} must be a contiguous int32 tensor of {n} (got {t.dtype} {tuple(t.shape)})")
+
+
+def _paged_kv(op: str, K, V, Ks, Vs, block_table, seq_lens):
+    """Checks a paged cache (tensors of one GPU); returns (packed descriptor, B, Hkv, D, tokens a sequence can hold)."""
     shape = K.shape
     if len(shape) != 4 or V.shape != shape:
         _fail(op, "shape", "K and V must both be [num_pages, Hkv, page_size, D]")
-    int8 = Ks is not None or Vs is not None
-    code = torch.int8 if int8 else torch.float16
+    code = _F16 if Ks is None else _I8
     if K.dtype is not code or V.dtype is not code:
-        _fail(op, "int8" if int8 else "fp16", f"K and V must be {code} (got {K.dtype}, {V.dtype})")
+        _fail(op, "fp16" if Ks is None else "int8", f"K and V must be {code} (got {K.dtype}, {V.dtype})")
     P, Hkv, page, D = shape
-    sk, sv = K.stride(), V.stride()
+    k0, k1, k2, k3 = K.stride()
+    v0, v1, v2, v3 = V.stride()
     if D != 64 and D != 128:
         _fail(op, "D", f"head_dim must be 64 or 128 (got {D})")
-    if sk[3] != 1 or sv[3] != 1:
+    if k3 != 1 or v3 != 1:
         _fail(op, "stride", "K and V must be contiguous over D")
-    _index_tensor(op, "block_table", block_table, dev)
-    if block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        _fail(op, "block_table", "block_table must be [B, max_pages] with contiguous rows")
-    B, max_pages = block_table.shape
+    tshape = block_table.shape
+    if len(tshape) != 2 or block_table.dtype is not _I32:
+        _fail(op, "block_table", "block_table must be an int32 [B, max_pages] tensor")
+    B, max_pages = tshape
+    t0, t1 = block_table.stride()
+    if t1 != 1 and max_pages > 1:
+        _fail(op, "block_table", "block_table must have contiguous rows")
     lens = 0
     if seq_lens is not None:
-        _index_vector(op, "seq_lens", seq_lens, B, dev)
+        _index_vector(op, "seq_lens", seq_lens, B)
         lens = seq_lens.data_ptr()
-    ks = vs = 0
-    sks = svs = (0, 0)
-    if int8:
-        _require_cuda(op, K, Ks, Vs)
-        _require_dtype(op, "fp16", torch.float16, Ks=Ks, Vs=Vs)
-        if Ks.shape != shape[:3] or Vs.shape != shape[:3]:
-            _fail(op, "shape", f"Ks and Vs must be [num_pages, Hkv, page_size] = {tuple(shape[:3])}")
-        sks, svs = Ks.stride(), Vs.stride()
-        if sks[2] != 1 or svs[2] != 1:
+    ks = vs = ks0 = ks1 = vs0 = vs1 = fmt = 0
+    if Ks is not None:
+        fmt = _native.KV_INT8
+        if Ks.dtype is not _F16 or Vs.dtype is not _F16:
+            _fail(op, "fp16", f"Ks and Vs must be {_F16} (got {Ks.dtype}, {Vs.dtype})")
+        if Ks.shape != (P, Hkv, page) or Vs.shape != (P, Hkv, page):
+            _fail(op, "shape", f"Ks and Vs must be [num_pages, Hkv, page_size] = {(P, Hkv, page)}")
+        ks0, ks1, ks2 = Ks.stride()
+        vs0, vs1, vs2 = Vs.stride()
+        if ks2 != 1 or vs2 != 1:
             _fail(op, "stride", "Ks and Vs must be contiguous over a page's tokens")
         ks, vs = Ks.data_ptr(), Vs.data_ptr()
-    desc = _native.PAGED_KV.pack(
-        _native.KV_INT8 if int8 else _native.KV_F16, 0, page, P, max_pages, B, Hkv, D, K.data_ptr(), V.data_ptr(), ks, vs,
-        sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], sks[0], sks[1], svs[0], svs[1], block_table.data_ptr(),
-        block_table.stride(0), lens)
-    return desc, B, Hkv, D, max_pages * page, int8
+    desc = _native.PAGED_KV.pack(fmt, 0, page, P, max_pages, B, Hkv, D, K.data_ptr(), V.data_ptr(), ks, vs, k0, k1, k2, v0,
+                                 v1, v2, ks0, ks1, vs0, vs1, block_table.data_ptr(), t0, lens)
+    return desc, B, Hkv, D, max_pages * page
 
 
-def _scratch(op: str, workspace, nbytes: int, dev: torch.device):
-    """The caller's workspace, checked, or a new one from torch's allocator: (pointer, bytes, tensor to keep)."""
-    if workspace is None:
-        if not nbytes:
-            return None, 0, None
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        return workspace.data_ptr(), nbytes, workspace
-    if not isinstance(workspace, torch.Tensor) or workspace.device != dev or not workspace.is_contiguous():
+def _scales(op: str, Ks, Vs) -> tuple:
+    """The scale tensors among a call's inputs: none or both."""
+    if (Ks is None) != (Vs is None):
+        _fail(op, "fp16", "Ks and Vs go together")
+    return () if Ks is None else (Ks, Vs)
+
+
+def _scratch(op: str, workspace: torch.Tensor, idx: int):
+    """(pointer, bytes) of the caller's workspace."""
+    if not isinstance(workspace, torch.Tensor) or workspace.get_device() != idx or not workspace.is_contiguous():
         _fail(op, "workspace", "workspace must be a contiguous tensor on the inputs' device")
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
-def _slot_weights(op: str, name: str, w, shape, dev: torch.device) -> None:
-    if not isinstance(w, torch.Tensor) or w.device != dev or w.dtype != torch.float32 or not w.is_contiguous() \
-            or w.shape != shape:
-        _fail(op, name, f"{name} must be a contiguous float32 {list(shape)} tensor on the inputs' device")
+def _slot_weights(op: str, name: str, w, shape) -> None:
+    if w.dtype is not _F32 or w.shape != shape or not w.is_contiguous():
+        _fail(op, name, f"{name} must be a contiguous float32 {list(shape)} tensor (got {w.dtype} {tuple(w.shape)})")
+
+
+# Workspace sizes by (GPU, arguments): they depend on nothing else.
+_workspace_sizes: dict = {}
+
+
+def _workspace_size(idx: int, fn, *args) -> int:
+    key = (idx, fn, *args)
+    n = _workspace_sizes.get(key)
+    if n is None:
+        n = int(_on_gpu(idx, getattr(_native.lib(), fn), *args))
+        if len(_workspace_sizes) >= 1024:
+            _workspace_sizes.clear()
+        if n:  # 0: refused, the call itself says why
+            _workspace_sizes[key] = n
+    return n
 
 
 def paged_workspace_bytes(kv_format: str, B: int, Hq: int, Hkv: int, max_len: int, D: int, weights: bool = False) -> int:
@@ -864,26 +908,34 @@ def evict_workspace_bytes(B: int, Hkv: int, max_len: int, budget: int) -> int:
 
 
 def _decode_paged(op, q, K, V, Ks, Vs, block_table, seq_lens, out, workspace, weights):
-    ts = (q, K, V, block_table, seq_lens)
-    dev = _require_cuda(op, *ts)
-    if q.dim() != 3 or q.dtype != torch.float16 or not q.is_contiguous():
+    ts = (q, K, V, block_table, seq_lens) + (() if Ks is None else (Ks, Vs))
+    idx = _gpu_of(op, *ts) if weights is None else _gpu_of(op, *ts, weights)
+    desc, B, Hkv, D, cap = _paged_kv(op, K, V, Ks, Vs, block_table, seq_lens)
+    qshape = q.shape
+    if len(qshape) != 3 or q.dtype is not _F16 or not q.is_contiguous():
         _fail(op, "fp16", "q must be a contiguous fp16 [B, Hq, D] tensor")
-    desc, B, Hkv, D, cap, int8 = _paged_kv(op, K, V, Ks, Vs, block_table, seq_lens, dev)
-    Hq = q.shape[1]
-    if q.shape[0] != B or q.shape[2] != D:
-        _fail(op, "shape", f"q has shape {tuple(q.shape)}, expected ({B}, Hq, {D})")
+    Hq = qshape[1]
+    if qshape[0] != B or qshape[2] != D:
+        _fail(op, "shape", f"q has shape {tuple(qshape)}, expected ({B}, Hq, {D})")
+    w = None
     if weights is not None:
-        _slot_weights(op, "weights", weights, (B, Hkv, cap), dev)
-    out = torch.empty_like(q) if out is None else _kv_out(op, q, out, q.shape, dev)
-    lib = _native.lib()
-    with _DeviceGuard(dev):
-        need = 0
-        if workspace is None:
-            need = lib.fqkv_paged_workspace_bytes(_native.KV_INT8 if int8 else _native.KV_F16, B, Hq, Hkv, D, cap,
-                                                  0 if weights is None else 1)
-        ws, nb, keep = _scratch(op, workspace, need, dev)
-        rc = lib.fqkv_decode_attn_paged(desc, 1 if out.dtype == torch.bfloat16 else 0, q.data_ptr(), out.data_ptr(), Hq,
-                                        None if weights is None else weights.data_ptr(), ws, nb, _stream(dev))
+        _slot_weights(op, "weights", weights, (B, Hkv, cap))
+        w = weights.data_ptr()
+    bf16 = 0
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _kv_out(op, q, out, qshape, q.device)
+        bf16 = 1 if out.dtype is _BF16 else 0
+    if workspace is None:
+        nb = _workspace_size(idx, "fqkv_paged_workspace_bytes", 0 if Ks is None else _native.KV_INT8, B, Hq, Hkv, D, cap,
+                             0 if w is None else 1)
+        workspace = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
+        ws = workspace.data_ptr() if nb else None
+    else:
+        ws, nb = _scratch(op, workspace, idx)
+    rc = _on_gpu(idx, _native.lib().fqkv_decode_attn_paged, desc, bf16, q.data_ptr(), out.data_ptr(), Hq, w, ws, nb,
+                 _stream_of(idx))
     if rc:
         _native.check(rc, f"launch: {op}")
     return out
@@ -951,41 +1003,48 @@ def rope_qkv_append_paged(qkv: torch.Tensor, cos_table: torch.Tensor, sin_table:
     :func:`check_device_status`; two tokens of one call must not share a slot.
     """
     op = "rope_qkv_append_paged"
-    dev = _require_cuda(op, qkv, cos_table, sin_table, positions, slots, block_table, q_out, K, V)
-    if qkv.dtype not in (torch.float16, torch.bfloat16):
+    ts = (qkv, cos_table, sin_table, positions, slots, block_table, q_out, K, V) + _scales(op, Ks, Vs)
+    if axes is not None:
+        ts += (axes,)
+    if seq_ids is not None:
+        ts += (seq_ids,)
+    idx = _gpu_of(op, *ts)
+    desc, B, Hkv, D, _ = _paged_kv(op, K, V, Ks, Vs, block_table, None)
+    bf16 = 1 if qkv.dtype is _BF16 else 0
+    if not bf16 and qkv.dtype is not _F16:
         _fail(op, "dtype", "qkv must be fp16 or bf16")
-    if qkv.dim() != 2 or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
-        _fail(op, "shape", "qkv must be [T, W] with contiguous rows")
-    if q_out.dim() != 3 or q_out.dtype != torch.float16 or not q_out.is_contiguous():
+    oshape, xshape = q_out.shape, qkv.shape
+    if len(oshape) != 3 or q_out.dtype is not _F16 or not q_out.is_contiguous():
         _fail(op, "fp16", "q_out must be a contiguous fp16 [T, Hq, D] tensor")
-    desc, B, Hkv, D, _, _ = _paged_kv(op, K, V, Ks, Vs, block_table, None, dev)
-    T, Hq = q_out.shape[:2]
-    if q_out.shape[2] != D or qkv.shape[0] != T or qkv.shape[1] < (Hq + 2 * Hkv) * D:
-        _fail(op, "shape", f"qkv must be [T, >= (Hq + 2 Hkv) D] and q_out [T, Hq, {D}] "
-                           f"(got {tuple(qkv.shape)}, {tuple(q_out.shape)})")
-    rows = cos_table.shape[0] if cos_table.dim() else 0
-    if cos_table.shape != (rows, D // 2) or sin_table.shape != (rows, D // 2) or cos_table.dtype is not torch.float32 \
-            or sin_table.dtype is not torch.float32 or not cos_table.is_contiguous() or not sin_table.is_contiguous():
+    T, Hq, oD = oshape
+    width = (Hq + 2 * Hkv) * D
+    if oD != D or len(xshape) != 2 or xshape[0] != T or xshape[1] < width or qkv.stride(1) != 1:
+        _fail(op, "shape", f"qkv must be [T, >= (Hq + 2 Hkv) D] with contiguous rows and q_out [T, Hq, {D}] "
+                           f"(got {tuple(xshape)}, {tuple(oshape)})")
+    tshape = cos_table.shape
+    if len(tshape) != 2 or tshape[1] != D // 2 or sin_table.shape != tshape or cos_table.dtype is not _F32 \
+            or sin_table.dtype is not _F32 or not cos_table.is_contiguous() or not sin_table.is_contiguous():
         _fail(op, "tables", f"cos_table and sin_table must be contiguous float32 [rows, D/2 = {D // 2}]")
-    _index_vector(op, "slots", slots, T, dev)
-    _index_tensor(op, "positions", positions, dev)
-    if positions.dim() not in (1, 2) or positions.shape[-1] != T or (T > 1 and positions.stride(-1) != 1):
-        _fail(op, "positions", f"positions must be [T = {T}] or [A, T] with contiguous rows")
-    A = positions.shape[0] if positions.dim() == 2 else 1
+    _index_vector(op, "slots", slots, T)
+    pshape = positions.shape
+    if positions.dtype is not _I32 or len(pshape) not in (1, 2) or pshape[-1] != T or (T > 1 and positions.stride(-1) != 1):
+        _fail(op, "positions", f"positions must be int32 [T = {T}] or [A, T] with contiguous rows")
+    A = pshape[0] if len(pshape) == 2 else 1
+    amap, astride = None, T
     if A > 1:
         if axes is None:
             _fail(op, "axes", "several position axes need axes [D/2]")
-        _index_vector(op, "axes", axes, D // 2, dev)
+        _index_vector(op, "axes", axes, D // 2)
+        amap, astride = axes.data_ptr(), positions.stride(0)
+    ids = None
     if seq_ids is not None:
-        _index_vector(op, "seq_ids", seq_ids, T, dev)
-    with _DeviceGuard(dev):
-        rc = _native.lib().fqkv_rope_append_paged(
-            desc, 1 if qkv.dtype == torch.bfloat16 else 0, qkv.data_ptr(),
-            qkv.stride(0) if T > 1 else (Hq + 2 * Hkv) * D, cos_table.data_ptr(),
-            sin_table.data_ptr(), rows, positions.data_ptr(), positions.stride(0) if A > 1 else T, A,
-            axes.data_ptr() if A > 1 else None, None if seq_ids is None else seq_ids.data_ptr(), slots.data_ptr(),
-            q_out.data_ptr(), T, Hq, _stream(dev))
-    _native.check(rc, f"launch: {op}")
+        _index_vector(op, "seq_ids", seq_ids, T)
+        ids = seq_ids.data_ptr()
+    rc = _on_gpu(idx, _native.lib().fqkv_rope_append_paged, desc, bf16, qkv.data_ptr(), qkv.stride(0) if T > 1 else width,
+                 cos_table.data_ptr(), sin_table.data_ptr(), tshape[0], positions.data_ptr(), astride, A, amap, ids,
+                 slots.data_ptr(), q_out.data_ptr(), T, Hq, _stream_of(idx))
+    if rc:
+        _native.check(rc, f"launch: {op}")
 
 
 def evict_kvcache_paged(K: torch.Tensor, V: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -1003,24 +1062,31 @@ def evict_kvcache_paged(K: torch.Tensor, V: torch.Tensor, block_table: torch.Ten
     sequences must be copied first.  ``workspace``: ``evict_workspace_bytes`` bytes, allocated when not given.
     """
     op = "evict_kvcache_paged"
-    dev = _require_cuda(op, K, V, block_table, seq_lens, weights)
-    desc, B, Hkv, D, cap, _ = _paged_kv(op, K, V, Ks, Vs, block_table, seq_lens, dev)
-    _slot_weights(op, "weights", weights, (B, Hkv, cap), dev)
+    ts = (K, V, block_table, seq_lens, weights) + _scales(op, Ks, Vs)
+    if weights_out is not None:
+        ts += (weights_out,)
+    if lens_out is not None:
+        ts += (lens_out,)
+    idx = _gpu_of(op, *ts)
+    desc, B, Hkv, D, cap = _paged_kv(op, K, V, Ks, Vs, block_table, seq_lens)
+    _slot_weights(op, "weights", weights, (B, Hkv, cap))
     if weights_out is None:
         weights_out = weights
     else:
-        _slot_weights(op, "weights_out", weights_out, (B, Hkv, cap), dev)
+        _slot_weights(op, "weights_out", weights_out, (B, Hkv, cap))
     if lens_out is None:
         lens_out = torch.empty_like(seq_lens)
     else:
-        _index_vector(op, "lens_out", lens_out, B, dev)
-    lib = _native.lib()
-    with _DeviceGuard(dev):
-        need = 0
-        if workspace is None and B:
-            need = lib.fqkv_evict_workspace_bytes(B, Hkv, cap, int(budget))
-        ws, nb, keep = _scratch(op, workspace, need, dev)
-        rc = lib.fqkv_evict_paged(desc, weights.data_ptr(), weights_out.data_ptr(), lens_out.data_ptr(), int(budget),
-                                  int(recent), ws, nb, _stream(dev))
-    _native.check(rc, f"launch: {op}")
+        _index_vector(op, "lens_out", lens_out, B)
+    budget = int(budget)
+    if workspace is None:
+        nb = _workspace_size(idx, "fqkv_evict_workspace_bytes", B, Hkv, cap, budget) if B else 0
+        workspace = torch.empty(nb, dtype=torch.uint8, device=K.device) if nb else None
+        ws = workspace.data_ptr() if nb else None
+    else:
+        ws, nb = _scratch(op, workspace, idx)
+    rc = _on_gpu(idx, _native.lib().fqkv_evict_paged, desc, weights.data_ptr(), weights_out.data_ptr(), lens_out.data_ptr(),
+                 budget, int(recent), ws, nb, _stream_of(idx))
+    if rc:
+        _native.check(rc, f"launch: {op}")
     return lens_out
