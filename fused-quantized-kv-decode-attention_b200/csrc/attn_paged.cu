@@ -70,7 +70,7 @@ struct Cfg {
   static constexpr int kCtas = D == 128 ? 2 : (kI8 ? 3 : 4);
   static constexpr int kStages = 3;
   static constexpr size_t kRingBytes = size_t(kStages) * kStageBytes;
-  static constexpr size_t kBarBytes = 2 * kStages * sizeof(uint64_t);
+  static constexpr size_t kBarBytes = (2 * kStages * sizeof(uint64_t) + 15) & ~size_t(15);
   static constexpr int kHeadStride = D + 4;               // floats; makes the epilogue's stores conflict-free
   static constexpr size_t kMergeBytes = size_t(kWarps) * (2 * kPagedMaxHeads + kMergeHeads * kHeadStride) * sizeof(float);
   static constexpr size_t kSmemBytes = 1024 + kRingBytes + kBarBytes + kMergeBytes;
@@ -205,6 +205,12 @@ __device__ __forceinline__ void store_out(const PagedLaunch& a, size_t idx, floa
   else static_cast<__half*>(a.out)[idx] = __float2half_rn(v);
 }
 
+// Elements idx and idx + 1 (idx even; out is 4-byte aligned).
+__device__ __forceinline__ void store_out2(const PagedLaunch& a, size_t idx, float v0, float v1) {
+  if (a.out_bf16) *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + idx) = __floats2bfloat162_rn(v0, v1);
+  else *reinterpret_cast<__half2*>(static_cast<__half*>(a.out) + idx) = __floats2half2_rn(v0, v1);
+}
+
 // Two bytes of x (code + 128) as the fp16 numbers 1152 + code.
 template <uint32_t kSel>
 __device__ __forceinline__ uint32_t codes_to_half2(uint32_t x) {
@@ -246,7 +252,7 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
   uint8_t* smem = smem_raw + ((uint32_t(1024) - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kRingBytes);
   uint64_t* empty = full + C::kStages;
-  float* sm_m = reinterpret_cast<float*>(empty + C::kStages);  // [warps][kPagedMaxHeads]
+  float* sm_m = reinterpret_cast<float*>(smem + C::kRingBytes + C::kBarBytes);  // [kPagedMaxHeads][warps]
   float* sm_l = sm_m + kWarps * kPagedMaxHeads;
   float* sm_o = sm_l + kWarps * kPagedMaxHeads;                // [warps][kMergeHeads][kHeadStride]
   __shared__ int abort_flag;
@@ -662,8 +668,8 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
       if (t4 == 0) {
-        sm_m[warp * kPagedMaxHeads + g + 8 * nt] = m_run[nt];
-        sm_l[warp * kPagedMaxHeads + g + 8 * nt] = l;
+        sm_m[(g + 8 * nt) * kWarps + warp] = m_run[nt];
+        sm_l[(g + 8 * nt) * kWarps + warp] = l;
       }
     }
     for (int hp = 0; hp < gvalid; hp += kMergeHeads) {
@@ -683,28 +689,40 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
         }
       }
       named_bar_sync(1, 32 * kWarps);
-      const int nh = min(kMergeHeads, gvalid - hp);
-      for (int idx = ct; idx < nh * D; idx += 32 * kWarps) {
-        const int hl = idx / D, d = idx - hl * D;
-        const int hh = hp + hl;
-        float M = -INFINITY;
+      // a warp per head, D / 32 dimensions per lane
+      static_assert(kMergeHeads == kWarps, "one head of a pass per warp");
+      const int hh = hp + warp;
+      if (hh < gvalid) {
+        constexpr int kDims = D / 32;
+        const float4 m4 = *reinterpret_cast<const float4*>(sm_m + hh * kWarps);
+        const float4 l4 = *reinterpret_cast<const float4*>(sm_l + hh * kWarps);
+        const float M = fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w));
+        // a warp whose keys all lie past the last token has no say (its sums are 0; a NaN there stays a NaN)
+        auto weight = [&](float m) { return m == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : ex2(m - M); };
+        const float wt[kWarps] = {weight(m4.x), weight(m4.y), weight(m4.z), weight(m4.w)};
+        const float L = wt[0] * l4.x + wt[1] * l4.y + wt[2] * l4.z + wt[3] * l4.w;
+        float O[kDims];
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w * kPagedMaxHeads + hh]);
-        float L = 0.f, O = 0.f;
+        for (int i = 0; i < kDims; ++i) O[i] = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float mw = sm_m[w * kPagedMaxHeads + hh];
-          // a warp whose keys all lie past the last token has no say (its sums are 0; a NaN there stays a NaN)
-          const float wt = (mw == -INFINITY) ? (M == -INFINITY ? 1.f : 0.f) : ex2(mw - M);
-          L += wt * sm_l[w * kPagedMaxHeads + hh];
-          O += wt * sm_o[(w * kMergeHeads + hl) * C::kHeadStride + d];
+          const float* src = sm_o + (w * kMergeHeads + warp) * C::kHeadStride + lane * kDims;
+          float v[kDims];
+          if constexpr (kDims == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+          else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+#pragma unroll
+          for (int i = 0; i < kDims; ++i) O[i] += wt[w] * v[i];
         }
         if (whole) {
-          store_out(a, (row_base + hh) * D + d, O / L);
-          if (d == 0 && a.scores) a.row_ml[row_base + hh] = make_float2(M, L);
+          const float r = 1.f / L;
+#pragma unroll
+          for (int i = 0; i < kDims; i += 2) store_out2(a, (row_base + hh) * D + lane * kDims + i, O[i] * r, O[i + 1] * r);
+          if (lane == 0 && a.scores) a.row_ml[row_base + hh] = make_float2(M, L);
         } else {
-          if (d == 0) a.part_ml[slot * a.GP + hh] = make_float2(M, L);
-          a.part_o[(slot * a.GP + hh) * D + d] = O;
+          if (lane == 0) a.part_ml[slot * a.GP + hh] = make_float2(M, L);
+          float* dst = a.part_o + (slot * a.GP + hh) * D + lane * kDims;
+          if constexpr (kDims == 4) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(O);
+          else *reinterpret_cast<float2*>(dst) = *reinterpret_cast<const float2*>(O);
         }
       }
       named_bar_sync(1, 32 * kWarps);

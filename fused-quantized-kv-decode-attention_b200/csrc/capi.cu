@@ -913,8 +913,8 @@ static int paged_cache(const fqkv_paged_kv_t* kv, bool need_lens, fqkv::PagedCac
                 (long long)kv->B, (long long)kv->Hkv, (long long)kv->num_pages, (long long)kv->max_pages);
   constexpr int64_t kMax = INT32_MAX;
   if (kv->num_pages >= kMax || kv->page_size > kMax || kv->Hkv > 65535 || kv->B > 65535 || kv->B * kv->Hkv > 65535 ||
-      kv->max_pages > kMax / kv->page_size)
-    return fail(FQKV_ERR_INVALID_ARGUMENT, "sizes exceed the index range (B * Hkv <= 65535, max_pages * page_size < 2^31)");
+      kv->max_pages > (int64_t(1) << 30) / kv->page_size)
+    return fail(FQKV_ERR_INVALID_ARGUMENT, "sizes exceed the index range (B * Hkv <= 65535, max_pages * page_size <= 2^30)");
   if (kv->B == 0) return FQKV_OK;
   if (!kv->k || !kv->v || !kv->block_table || (need_lens && !kv->seq_lens) || (int8 && (!kv->k_scales || !kv->v_scales)))
     return fail(FQKV_ERR_INVALID_ARGUMENT, "null tensor pointer");

@@ -351,7 +351,7 @@ int fqkv_argmax(int32_t model_dtype, const void* logits, int64_t rows, int64_t V
  * entries past a sequence's last page, and pool slots past its last token,
  * may hold anything.  A needed entry outside [0, num_pages) is never
  * followed: status 65 is recorded (fqkv_device_status) and that sequence's
- * result is undefined.  B * Hkv <= 65535. */
+ * result is undefined.  B * Hkv <= 65535, max_pages * page_size <= 2^30. */
 typedef struct fqkv_paged_kv {
   int32_t kv_format;           /* FQKV_KV_F16 or FQKV_KV_INT8 */
   int32_t reserved;

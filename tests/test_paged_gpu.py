@@ -137,7 +137,8 @@ def test_attention_head_layouts(fqkv, int8, Hq, Hkv, D):
 
 
 @pytest.mark.parametrize("int8", [False, True])
-@pytest.mark.parametrize("lens", [[5000], [4097, 1], [1, 0, 0, 2500], [0, 0, 0], [3] * 70 + [0] * 40 + [700] + [64] * 200])
+@pytest.mark.parametrize("lens", [[5000], [4097, 1], [1, 0, 0, 2500], [0, 0, 0], [3] * 70 + [0] * 40 + [700] + [64] * 200,
+                                  [0] * 300 + [130] + [1] * 555 + [0, 65]])
 def test_attention_splits_and_batches(fqkv, int8, lens):
     """Units that cross many CTAs, and batches past one warp's scan, with and without the weights."""
     c = Cache(fqkv, lens, 1 if len(lens) > 9 else 2, 64, 32, int8, seed=len(lens))
