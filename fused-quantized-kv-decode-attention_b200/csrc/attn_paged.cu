@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
         }
       } else {
         uint2 raw[2 * kQS];
-        uint32_t top = 0;  // largest magnitude, as bits: inf and NaN stand above all numbers
+        __half2 top2 = __half2half2(__ushort_as_half(0));  // largest magnitude; a NaN stays one
 #pragma unroll
         for (int i = 0; i < 2 * kQS; ++i) {
           raw[i] = make_uint2(0u, 0u);
@@ -405,10 +405,16 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
             raw[i].x = *reinterpret_cast<const uint32_t*>(qrow + 16 * i + 4 * t4);
             raw[i].y = *reinterpret_cast<const uint32_t*>(qrow + 16 * i + 4 * t4 + 2);
           }
-          top = max(top, max(max(raw[i].x & 0x7fffu, (raw[i].x >> 16) & 0x7fffu), max(raw[i].y & 0x7fffu, (raw[i].y >> 16) & 0x7fffu)));
         }
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+#pragma unroll
+        for (int i = 0; i < 2 * kQS; ++i) {
+          top2 = __hmax2_nan(top2, __habs2(*reinterpret_cast<const __half2*>(&raw[i].x)));
+          top2 = __hmax2_nan(top2, __habs2(*reinterpret_cast<const __half2*>(&raw[i].y)));
+        }
+        top2 = __hmax2_nan(top2, __shfl_xor_sync(0xffffffffu, top2, 1));
+        top2 = __hmax2_nan(top2, __shfl_xor_sync(0xffffffffu, top2, 2));
+        const __half top1 = __hmax_nan(__low2half(top2), __high2half(top2));
+        const uint32_t top = __half_as_ushort(top1) & 0x7fffu;  // inf and NaN: 0x7c00 and above
         // 2^k = 2^(21 - floor(log2 max |q|)), by the exponent field
         const int e = top == 0u ? 127 : (__float_as_int(__half2float(__ushort_as_half(uint16_t(top)))) >> 23);
         const float unit = __int_as_float((127 + 21 + 127 - e) << 23);
