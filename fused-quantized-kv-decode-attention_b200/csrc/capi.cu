@@ -1175,6 +1175,7 @@ int fqkv_evict_paged(const fqkv_paged_kv_t* kv, const float* weights, float* wei
   a.lens_out = reinterpret_cast<int*>(lens_out);
   a.state = static_cast<int2*>(workspace);
   a.list = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + pad256(size_t(units) * sizeof(int2)));
+  a.sms = ds->sm_count;
   a.status = ds->status;
   cudaError_t e = fqkv::launch_evict_paged(a, reinterpret_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "eviction launch");

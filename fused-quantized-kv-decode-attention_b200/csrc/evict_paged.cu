@@ -12,13 +12,14 @@
 // 15 us, 58 % of the issue slots); in a cluster the CTAs add their few used bins to the first one's by
 // distributed-shared-memory atomics, integers, so the order does not matter.
 //
-// The move: bound by HBM, 2 x the kept rows (48 sequences of 16K -> 4096, D = 128, fp16: 1.65 GB in 369 us, selection
+// The move: bound by HBM, 2 x the kept rows (48 sequences of 16K -> 4096, D = 128, fp16: 1.65 GB in 332 us, selection
 // included).  In place, and the list is ascending with list[p] >= p: a row's
 // destination is at or before its source.  One CTA moves one column slice of K (or V) of one (sequence, KV
 // head), chunk by chunk in list order; a chunk is written only after it and all earlier chunks were read, and a
 // chunk's writes end below the next chunk's first source, so reading ahead is free.  Slices make enough CTAs for
 // few sequences.  The chunks before the first gap are not touched.  32 KB chunks, three in flight: chunks of
-// 16 KB are as fast for 16 x 16K and slower for long moves (4 x 100000 -> 50000: 555 us instead of 457 us).
+// 16 KB take 411 us for 4 x 100000 -> 50000 instead of 357 us.  (One launch, with a cluster per (sequence, KV head) that
+// selects and then moves, was 5 us slower for one sequence -- a cluster's barriers -- and no faster for many.)
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -299,8 +300,8 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
 }
 
 // ------------------------------------------------------------------ the move
-constexpr int kMoveThreads = 256;
-constexpr int kMoveVecs = 8;                                // 16-byte pieces per thread and chunk
+constexpr int kMoveThreads = 512;
+constexpr int kMoveVecs = 4;                                // 16-byte pieces per thread and chunk
 constexpr int kMoveStages = 3;                              // chunks in flight per CTA
 constexpr int kChunkVecs = kMoveThreads * kMoveVecs;
 
@@ -499,11 +500,12 @@ cudaError_t evict_prepare() {
 cudaError_t launch_evict_paged(const PagedEvict& args, cudaStream_t stream) {
   PagedEvict a = args;
   const int units = a.kv.B * a.kv.Hkv;
-  // The move: column slices until about 1000 CTAs exist, none narrower than a 32-byte sector.  16 sequences of
-  // 0 to 16K tokens -> 4096, 8 KV heads, D = 128: 2 slices 123 us, 4 slices 111 us, 8 slices 134 us (pieces of
-  // one 64-byte DRAM access fetched at different times).
+  // The move: column slices until about 500 CTAs exist, none narrower than 64 bytes (a DRAM access: 4 sequences of
+  // 100000 -> 50000, 8 KV heads, D = 128: 4 slices of 64 bytes 357 us, 8 of 32 bytes 482 us); 32 bytes only where there
+  // would not be a CTA per SM (one sequence of 16K -> 4096: 34 us in 64, 28 us in 128 CTAs).
   a.slices = 1;
-  while (units * 2 * a.slices < 1024 && a.kv.D * (a.kv.int8 ? 1 : 2) / a.slices > 32) a.slices *= 2;
+  const auto width = [&] { return a.kv.D * (a.kv.int8 ? 1 : 2) / a.slices; };
+  while ((units * 2 * a.slices < 512 && width() > 64) || (units * 2 * a.slices < a.sms && width() > 32)) a.slices *= 2;
   // The selection: one CTA while a full sequence is about what it holds in registers (one step and a half, so that a
   // table with room to spare for 16K tokens does not pay a cluster's barriers: 31 us instead of 35 us for one such
   // sequence of 8 KV heads), then clusters of 2, 4 and 8.

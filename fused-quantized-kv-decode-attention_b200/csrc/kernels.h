@@ -276,6 +276,7 @@ struct PagedEvict {
   int* list;               // [B * Hkv][budget]: kept tokens in order (workspace)
   int budget, recent;
   int cluster, slices;     // chosen by the launch: selection CTAs per (sequence, KV head); column slices of a row
+  int sms;
   int* status;
 };
 cudaError_t evict_prepare();
