@@ -12,13 +12,13 @@
 // 15 us, 58 % of the issue slots); in a cluster the CTAs add their few used bins to the first one's by
 // distributed-shared-memory atomics, integers, so the order does not matter.
 //
-// The move: bound by HBM, 2 x the kept rows (48 sequences of 16K -> 4096, D = 128, fp16: 1.65 GB in 332 us, selection
+// The move: bound by HBM, 2 x the kept rows (48 sequences of 16K -> 4096, D = 128, fp16: 1.65 GB in 308 us, selection
 // included).  In place, and the list is ascending with list[p] >= p: a row's
 // destination is at or before its source.  One CTA moves one column slice of K (or V) of one (sequence, KV
 // head), chunk by chunk in list order; a chunk is written only after it and all earlier chunks were read, and a
 // chunk's writes end below the next chunk's first source, so reading ahead is free.  Slices make enough CTAs for
-// few sequences.  The chunks before the first gap are not touched.  32 KB chunks, three in flight: chunks of
-// 16 KB take 411 us for 4 x 100000 -> 50000 instead of 357 us.  (One launch, with a cluster per (sequence, KV head) that
+// few sequences.  The chunks before the first gap are not touched.  Two chunks of 32 KB in flight in each of three CTAs
+// per SM (three in each of two: 97 us instead of 95 us for 16 sequences; 16 KB chunks: 99 to 135 us).  (One launch, with a cluster per (sequence, KV head) that
 // selects and then moves, was 5 us slower for one sequence -- a cluster's barriers -- and no faster for many.)
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
 // ------------------------------------------------------------------ the move
 constexpr int kMoveThreads = 512;
 constexpr int kMoveVecs = 4;                                // 16-byte pieces per thread and chunk
-constexpr int kMoveStages = 3;                              // chunks in flight per CTA
+constexpr int kMoveStages = 2;                              // chunks in flight per CTA
 constexpr int kChunkVecs = kMoveThreads * kMoveVecs;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -312,10 +312,12 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// One column slice of one pool: v 16-byte pieces (a power of two) of every row.
+// One column slice of one pool: v 16-byte pieces (2, 4, 8 or 16) of every row.  The lanes of a warp share v lanes per
+// row, so each row's addresses are worked out by one lane (one or two rows per lane and chunk) and handed round:
+// computing them in every lane took 140 instructions per warp and 512 bytes, 61 % of the issue slots.
 __device__ void move_rows(const PagedEvict& a, const int* list, const int* row, uint8_t* base, int64_t page_stride,
                           int64_t tok_stride, int v, uint4* ring) {
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rows = kChunkVecs / v, shift = 31 - __clz(v);
   const int chunks = (a.budget + rows - 1) / rows;
   // the first chunk with a row that moves: list[p] == p holds up to the first gap and nowhere after it
@@ -328,37 +330,57 @@ __device__ void move_rows(const PagedEvict& a, const int* list, const int* row, 
     if (still < kMoveThreads) break;
   }
   const uint32_t my = smem_u32(ring) + tid * 16;
-  const int col = 16 * (tid & (v - 1));  // kMoveThreads is a multiple of v: the same piece of every row
-  const int row0 = tid >> shift, row_step = kMoveThreads >> shift;
+  const int col = 16 * (lane & (v - 1));
+  // piece i of a thread belongs to row i * row_step + tid / v of the chunk; a warp has 128 / v rows, numbered
+  // i * (32 / v) + lane / v; lane l looks after rows l and l + 32
+  const int per = 32 >> shift, warp_rows = kMoveVecs * per, row_step = kMoveThreads >> shift;
+  int mine[2];  // place in a chunk of this lane's rows; -1: none
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int s = lane + 32 * r;
+    mine[r] = s < warp_rows ? (s / per) * row_step + warp * per + s % per : -1;
+  }
+  auto hand = [&](unsigned long long x0, unsigned long long x1, int i) -> unsigned long long {
+    const int s = i * per + (lane >> shift);
+    return __shfl_sync(0xffffffffu, v == 2 && i >= kMoveVecs / 2 ? x1 : x0, s & 31);
+  };
+  static_assert(kMoveVecs == 4, "v = 2: pieces 0 and 1 lie in rows 0 .. 31, 2 and 3 in rows 32 .. 63");
   // Two steps ahead of the fetch of a chunk its list entries are read, one step ahead its pages.
-  int idx[kMoveVecs], page[kMoveVecs], off[kMoveVecs];
+  int idx[2], page[2], off[2];
   auto read_list = [&](int c) {
 #pragma unroll
-    for (int i = 0; i < kMoveVecs; ++i) {
-      const int p = c * rows + row0 + i * row_step;
-      idx[i] = p < a.budget ? list[p] : -1;  // (past the last chunk too)
+    for (int r = 0; r < 2; ++r) {
+      const int p = c * rows + mine[r];
+      idx[r] = mine[r] >= 0 && p < a.budget ? list[p] : -1;  // (past the last chunk too)
     }
   };
   auto read_pages = [&]() {
 #pragma unroll
-    for (int i = 0; i < kMoveVecs; ++i) {
-      page[i] = idx[i] < 0 ? 0 : row[a.kv.page_div.div(idx[i])];
-      off[i] = idx[i] < 0 ? -1 : a.kv.page_div.mod(idx[i]);  // -1: no row
+    for (int r = 0; r < 2; ++r) {
+      page[r] = idx[r] < 0 ? 0 : row[a.kv.page_div.div(idx[r])];
+      off[r] = idx[r] < 0 ? -1 : a.kv.page_div.mod(idx[r]);  // -1: no row
     }
   };
-  unsigned got = 0;  // which pieces of the chunks in flight were fetched, kMoveVecs bits per stage
-  static_assert(kMoveVecs * kMoveStages <= 32, "one bit per piece in flight");
+  // a row's address in the pool, 0 if its page is none of the pool's (recorded)
+  auto address = [&](int pg, int o) -> unsigned long long {
+    if (unsigned(pg) < unsigned(a.kv.num_pages))
+      return reinterpret_cast<unsigned long long>(base + pg * page_stride + o * tok_stride);
+    atomicCAS(a.status, kDevOk, kDevBadPage);
+    return 0ull;
+  };
+  unsigned got = 0;  // which of this lane's rows of the chunks in flight were fetched, 2 bits per stage
   auto fetch = [&](int st) {
-    got &= ~(((1u << kMoveVecs) - 1u) << (kMoveVecs * st));
+    got &= ~(3u << (2 * st));
+    unsigned long long src[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      src[r] = off[r] >= 0 ? address(page[r], off[r]) : 0ull;
+      if (src[r]) got |= 1u << (2 * st + r);
+    }
 #pragma unroll
     for (int i = 0; i < kMoveVecs; ++i) {
-      if (off[i] < 0) continue;
-      if (unsigned(page[i]) < unsigned(a.kv.num_pages)) {
-        cp_async16(my + (st * kChunkVecs + i * kMoveThreads) * 16, base + page[i] * page_stride + off[i] * tok_stride + col);
-        got |= 1u << (kMoveVecs * st + i);
-      } else {
-        atomicCAS(a.status, kDevOk, kDevBadPage);
-      }
+      const unsigned long long x = hand(src[0], src[1], i);
+      if (x) cp_async16(my + (st * kChunkVecs + i * kMoveThreads) * 16, reinterpret_cast<const uint8_t*>(x) + col);
     }
     cp_async_commit();
   };
@@ -371,28 +393,24 @@ __device__ void move_rows(const PagedEvict& a, const int* list, const int* row, 
     read_list(c + 2);
   }
   for (int c = first; c < chunks; ++c) {
-    int to_page[kMoveVecs];
-    const int p0 = c * rows + row0;
+    const int st = c % kMoveStages;
+    int to_page[2];
 #pragma unroll
-    for (int i = 0; i < kMoveVecs; ++i) {
-      const int p = p0 + i * row_step;
-      to_page[i] = p < a.budget ? row[a.kv.page_div.div(p)] : -1;
-    }
+    for (int r = 0; r < 2; ++r)
+      to_page[r] = (got >> (2 * st + r) & 1u) ? row[a.kv.page_div.div(c * rows + mine[r])] : 0;
     fetch((c + kMoveStages - 1) % kMoveStages);
     read_pages();
     read_list(c + kMoveStages + 1);
     cp_async_wait<kMoveStages - 1>();
     __syncthreads();  // the whole chunk (and all before it) is read: its destinations are free
-    const int st = c % kMoveStages;
+    unsigned long long dst[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      dst[r] = (got >> (2 * st + r) & 1u) ? address(to_page[r], a.kv.page_div.mod(c * rows + mine[r])) : 0ull;
 #pragma unroll
     for (int i = 0; i < kMoveVecs; ++i) {
-      if (!(got >> (kMoveVecs * st + i) & 1u)) continue;
-      if (unsigned(to_page[i]) >= unsigned(a.kv.num_pages)) {
-        atomicCAS(a.status, kDevOk, kDevBadPage);
-        continue;
-      }
-      uint8_t* dst = base + to_page[i] * page_stride + a.kv.page_div.mod(p0 + i * row_step) * tok_stride + col;
-      *reinterpret_cast<uint4*>(dst) = ring[st * kChunkVecs + tid + i * kMoveThreads];
+      const unsigned long long x = hand(dst[0], dst[1], i);
+      if (x) *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(x) + col) = ring[st * kChunkVecs + tid + i * kMoveThreads];
     }
   }
   cp_async_wait<0>();
@@ -500,12 +518,13 @@ cudaError_t evict_prepare() {
 cudaError_t launch_evict_paged(const PagedEvict& args, cudaStream_t stream) {
   PagedEvict a = args;
   const int units = a.kv.B * a.kv.Hkv;
-  // The move: column slices until about 500 CTAs exist, none narrower than 64 bytes (a DRAM access: 4 sequences of
+  // The move: column slices until about 600 CTAs exist, none narrower than 64 bytes (a DRAM access: 4 sequences of
   // 100000 -> 50000, 8 KV heads, D = 128: 4 slices of 64 bytes 357 us, 8 of 32 bytes 482 us); 32 bytes only where there
-  // would not be a CTA per SM (one sequence of 16K -> 4096: 34 us in 64, 28 us in 128 CTAs).
+  // would not be a CTA per SM (one sequence of 16K -> 4096: 34 us in 64, 28 us in 128 CTAs).  16 sequences of 0 to
+  // 16K -> 4096: 2 slices 95 us, 4 slices 90 us; 48 of 12K to 16K: 1 slice 308 us, 2 slices 322 us.
   a.slices = 1;
   const auto width = [&] { return a.kv.D * (a.kv.int8 ? 1 : 2) / a.slices; };
-  while ((units * 2 * a.slices < 512 && width() > 64) || (units * 2 * a.slices < a.sms && width() > 32)) a.slices *= 2;
+  while ((units * 2 * a.slices < 600 && width() > 64) || (units * 2 * a.slices < a.sms && width() > 32)) a.slices *= 2;
   // The selection: one CTA while a full sequence is about what it holds in registers (one step and a half, so that a
   // table with room to spare for 16K tokens does not pay a cluster's barriers: 31 us instead of 35 us for one such
   // sequence of 8 KV heads), then clusters of 2, 4 and 8.
