@@ -12,6 +12,8 @@
 // number of bytes whatever the lengths are.  A unit that lies inside one CTA's range is finished there; one
 // that crosses a border leaves unnormalised fp32 parts (two slots per CTA: the unit its range begins in and
 // the one it ends in), merged by the next launch in tile order, so results do not depend on timing.
+// Few short units (a choice of the host, by sizes) get a thread-block cluster each instead, which merges its parts
+// through distributed shared memory in the same launch.
 //
 //  * Warp 4 is the producer.  A tile is fetched as boxes of 16, 32, 64 or 128 keys (the largest that divides
 //    the page), each inside one page, by 4-D tensor copies over (D, token, head, page) with any 16-byte
@@ -52,6 +54,7 @@ namespace {
 constexpr int kWarps = 4;          // consumer warps
 constexpr int kThr = 32 * (kWarps + 1);
 constexpr int kMergeHeads = 4;     // heads merged per epilogue pass
+constexpr int kMaxCluster = 16;
 
 template <int D, bool kI8>
 struct Cfg {
@@ -171,6 +174,25 @@ struct Walk {
     }
   }
 
+  // One unit per cluster, its tiles shared out evenly over the cluster's CTAs.
+  __device__ __forceinline__ void init_cluster(const PagedLaunch& a, int tile_keys) {
+    lens = a.seq_lens;
+    B = a.B;
+    cap = a.cap;
+    tk = tile_keys;
+    groups = a.groups;
+    units_per_seq = a.Hkv * a.groups;
+    per = 0;
+    const int unit = int(blockIdx.x) / a.cluster, r = int(blockIdx.x) - unit * a.cluster;
+    b = unit / units_per_seq;
+    u = unit - b * units_per_seq;
+    len = length(b);
+    nt = tiles(len);
+    t = int(int64_t(nt) * r / a.cluster);
+    cur = 0;
+    end = int(int64_t(nt) * (r + 1) / a.cluster) - t;
+  }
+
   __device__ __forceinline__ bool next(Part& p) {
     if (cur >= end) return false;
     if (t >= nt) {  // past the unit: the next one, of the next sequence that has tokens
@@ -203,6 +225,12 @@ struct Walk {
 __device__ __forceinline__ void store_out(const PagedLaunch& a, size_t idx, float v) {
   if (a.out_bf16) static_cast<__nv_bfloat16*>(a.out)[idx] = __float2bfloat16_rn(v);
   else static_cast<__half*>(a.out)[idx] = __float2half_rn(v);
+}
+
+__device__ __forceinline__ float2 ld_dsmem_f32x2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
 }
 
 // Elements idx and idx + 1 (idx even; out is 4-byte aligned).
@@ -244,8 +272,9 @@ __device__ __forceinline__ void q_planes(const uint2& q, float f, uint32_t& hi, 
   hi = __byte_perm(__byte_perm(u0, u1, 0x0062), __byte_perm(u2, u3, 0x0062), 0x5410) ^ 0x80808080u;
 }
 
-// kNT: column tiles of 8 heads (1: up to 8 heads per unit, 2: up to 16).
-template <int D, bool kI8, int kNT>
+// kNT: column tiles of 8 heads (1: up to 8 heads per unit, 2: up to 16).  kCl: a thread-block cluster per unit, whose
+// CTAs merge their parts through distributed shared memory.
+template <int D, bool kI8, int kNT, bool kCl>
 __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(const __grid_constant__ PagedLaunch a) {
   using C = Cfg<D, kI8>;
   extern __shared__ uint8_t smem_raw[];
@@ -278,7 +307,8 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
   pdl_wait_primary();
 
   Walk walk;
-  walk.init(a, C::TK);
+  if constexpr (kCl) walk.init_cluster(a, C::TK);
+  else walk.init(a, C::TK);
   Part p;
 
   // ------------------------------------------------------------ producer
@@ -349,6 +379,11 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
           mbar_wait(&full[j % C::kStages], (j / C::kStages) & 1, wc, kDevTimeoutDrain);
       }
     }
+    if constexpr (kCl) {  // the whole warp takes part in the consumers' two cluster barriers
+      __syncwarp();
+      cluster_sync_all();
+      cluster_sync_all();
+    }
     return;
   }
 
@@ -366,8 +401,12 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
   bool alive = true;
   int it = 0;
 
+  // a cluster's CTA leaves its part here, in the ring, when all its tiles have been used
+  float* cl_ml = reinterpret_cast<float*>(smem);  // [kPagedMaxHeads][2]: maximum, sum
+  float* cl_o = cl_ml + 2 * kPagedMaxHeads;       // [kPagedMaxHeads][D]
+
   // sequences without tokens: zeros, and no parts
-  for (int b = int(blockIdx.x); b < a.B; b += int(gridDim.x))
+  for (int b = int(blockIdx.x); !kCl && b < a.B; b += int(gridDim.x))
     if (a.seq_lens[b] <= 0) {
       for (int i = ct; i < a.Hq * D; i += 32 * kWarps) store_out(a, size_t(b) * a.Hq * D + i, 0.f);
       const int units = a.Hkv * a.groups;
@@ -719,7 +758,12 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
 #pragma unroll
           for (int i = 0; i < kDims; ++i) O[i] += wt[w] * v[i];
         }
-        if (whole) {
+        if constexpr (kCl) {
+          if (lane == 0) *reinterpret_cast<float2*>(cl_ml + 2 * hh) = make_float2(M, L);
+          float* dst = cl_o + hh * D + lane * kDims;
+          if constexpr (kDims == 4) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(O);
+          else *reinterpret_cast<float2*>(dst) = *reinterpret_cast<const float2*>(O);
+        } else if (whole) {
           const float r = 1.f / L;
 #pragma unroll
           for (int i = 0; i < kDims; i += 2) store_out2(a, (row_base + hh) * D + lane * kDims + i, O[i] * r, O[i + 1] * r);
@@ -734,11 +778,50 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
       named_bar_sync(1, 32 * kWarps);
     }
     // the CTA that a unit begins in says in how many parts it comes, and from which CTA on
-    if (p.t0 == 0 && ct == 0 && a.unit_info) {
+    if (!kCl && p.t0 == 0 && ct == 0 && a.unit_info) {
       const int more = p.nt - p.t1;
       a.unit_info[(p.b * a.Hkv + p.kh) * a.groups + p.grp] =
           make_int2(int(blockIdx.x), more ? 1 + (more + walk.per - 1) / walk.per : 0);
     }
+  }
+  if constexpr (kCl) {
+    const int S = a.cluster, r = int(cluster_ctarank());
+    const int gvalid = min(a.GP, a.G - (walk.u % a.groups) * a.GP);
+    const size_t row_base = size_t(walk.b) * a.Hq + size_t(walk.u / a.groups) * a.G + size_t(walk.u % a.groups) * a.GP;
+    if (walk.end == 0 && ct < gvalid) *reinterpret_cast<float2*>(cl_ml + 2 * ct) = make_float2(-INFINITY, 0.f);  // no tiles
+    cluster_sync_all();
+    // the outputs, two dimensions at a time, shared out over the cluster; parts always in CTA order
+    for (int i = r * (32 * kWarps) + ct; i < gvalid * (D / 2); i += S * 32 * kWarps) {
+      const int hh = i / (D / 2), d = 2 * (i - hh * (D / 2));
+      const uint32_t ml_at = smem_u32(cl_ml + 2 * hh), o_at = smem_u32(cl_o + hh * D + d);
+      float2 ml[kMaxCluster], o[kMaxCluster];
+      float M = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < kMaxCluster; ++j) {
+        ml[j] = make_float2(-INFINITY, 0.f);
+        o[j] = make_float2(0.f, 0.f);
+        if (j < S) {
+          ml[j] = ld_dsmem_f32x2(dsmem_addr(ml_at, j));
+          o[j] = ld_dsmem_f32x2(dsmem_addr(o_at, j));
+        }
+        M = fmaxf(M, ml[j].x);
+      }
+      float L = 0.f;
+      float2 O = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < kMaxCluster; ++j) {
+        // no say: a CTA without tiles (its o was never written); sums of NaN scores have maximum -inf and stay
+        if (ml[j].x == -INFINITY && ml[j].y == 0.f) continue;
+        const float w = M == -INFINITY ? 1.f : ex2(ml[j].x - M);
+        L += w * ml[j].y;
+        O.x += w * o[j].x;
+        O.y += w * o[j].y;
+      }
+      const bool none = walk.len == 0;  // an empty sequence: zeros
+      store_out2(a, (row_base + hh) * D + d, none ? 0.f : O.x / L, none ? 0.f : O.y / L);
+      if (d == 0 && a.scores) a.row_ml[row_base + hh] = make_float2(M, L);
+    }
+    cluster_sync_all();  // nobody leaves while its part is read
   }
 }
 
@@ -894,38 +977,77 @@ __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(const __gr
   if (info.y) merge_unit<D>(a, info, unit, (int(blockIdx.x) - unit * per_unit) * a.merge_heads, sm_o, sm_ml);
 }
 
-template <int D, bool kI8, int kNT>
-const void* kernel_of() {
-  return reinterpret_cast<const void*>(&paged_attn_kernel<D, kI8, kNT>);
-}
-
 template <int D, bool kI8>
-cudaError_t prepare(int* ctas_per_sm) {
-  int n[2] = {0, 0};
+cudaError_t prepare(PagedOccupancy (&occ)[2]) {
+  constexpr size_t smem = Cfg<D, kI8>::kSmemBytes;
+  const void* fn[2][2] = {{reinterpret_cast<const void*>(&paged_attn_kernel<D, kI8, 1, false>),
+                           reinterpret_cast<const void*>(&paged_attn_kernel<D, kI8, 1, true>)},
+                          {reinterpret_cast<const void*>(&paged_attn_kernel<D, kI8, 2, false>),
+                           reinterpret_cast<const void*>(&paged_attn_kernel<D, kI8, 2, true>)}};
   for (int i = 0; i < 2; ++i) {
-    const void* fn = i ? kernel_of<D, kI8, 2>() : kernel_of<D, kI8, 1>();
-    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg<D, kI8>::kSmemBytes));
-    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n[i], fn, kThr, Cfg<D, kI8>::kSmemBytes);
+    cudaError_t e = cudaSuccess;
+    for (int cl = 0; cl < 2 && e == cudaSuccess; ++cl)
+      e = cudaFuncSetAttribute(fn[i][cl], cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(fn[i][1], cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ[i].ctas_per_sm, fn[i][0], kThr, smem);
     if (e != cudaSuccess) return e;
-    ctas_per_sm[i] = n[i];
+    for (int k = 0; k < 4; ++k) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(2u << k);
+      cfg.blockDim = dim3(kThr);
+      cfg.dynamicSmemBytes = smem;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 2u << k;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, fn[i][1], &cfg) != cudaSuccess) {
+        cudaGetLastError();  // an unsupported size is not an error of the library
+        n = 0;
+      }
+      occ[i].clusters[k] = n;
+    }
   }
   return cudaSuccess;
 }
 
+template <int D, bool kI8, int kNT>
+cudaError_t launch_nt(const PagedLaunch& a, cudaStream_t stream) {
+  constexpr size_t smem = Cfg<D, kI8>::kSmemBytes;
+  if (!a.cluster) return launch_pdl(paged_attn_kernel<D, kI8, kNT, false>, dim3(a.grid), dim3(kThr), smem, stream, a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.grid);
+  cfg.blockDim = dim3(kThr);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(a.cluster);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, paged_attn_kernel<D, kI8, kNT, true>, a);
+}
+
 template <int D, bool kI8>
 cudaError_t launch(const PagedLaunch& a, cudaStream_t stream) {
-  constexpr size_t smem = Cfg<D, kI8>::kSmemBytes;
-  return a.GP > 8 ? launch_pdl(paged_attn_kernel<D, kI8, 2>, dim3(a.grid), dim3(kThr), smem, stream, a)
-                  : launch_pdl(paged_attn_kernel<D, kI8, 1>, dim3(a.grid), dim3(kThr), smem, stream, a);
+  static_assert((2 * kPagedMaxHeads + kPagedMaxHeads * D) * sizeof(float) <= Cfg<D, kI8>::kRingBytes, "a part fits the ring");
+  return a.GP > 8 ? launch_nt<D, kI8, 2>(a, stream) : launch_nt<D, kI8, 1>(a, stream);
 }
 
 }  // namespace
 
 int paged_tile_keys(bool int8) { return int8 ? Cfg<128, true>::TK : Cfg<128, false>::TK; }
 
-cudaError_t paged_attn_prepare(bool int8, int D, int (&ctas_per_sm)[2]) {
-  if (int8) return D == 128 ? prepare<128, true>(ctas_per_sm) : prepare<64, true>(ctas_per_sm);
-  return D == 128 ? prepare<128, false>(ctas_per_sm) : prepare<64, false>(ctas_per_sm);
+cudaError_t paged_attn_prepare(bool int8, int D, PagedOccupancy (&occ)[2]) {
+  if (int8) return D == 128 ? prepare<128, true>(occ) : prepare<64, true>(occ);
+  return D == 128 ? prepare<128, false>(occ) : prepare<64, false>(occ);
 }
 
 cudaError_t launch_paged_attn(const PagedLaunch& a, cudaStream_t stream) {

@@ -222,6 +222,7 @@ struct PagedLaunch {
   int cap, num_pages, box;
   FastDiv page_div;
   int grid;
+  int cluster;             // 0, or the CTAs per unit, which form a thread-block cluster and merge their parts themselves
   // parts of units that cross a CTA's border; unit_info null: none can
   int2* unit_info;         // [B * Hkv * groups]: the CTA of the first part, the number of parts (0: none)
   float2* part_ml;         // [grid * 2][GP]
@@ -238,8 +239,12 @@ struct PagedLaunch {
   bool int8, out_bf16;
 };
 int paged_tile_keys(bool int8);
-// Resident CTAs per SM of the variants for up to 8 and up to 16 heads per unit.
-cudaError_t paged_attn_prepare(bool int8, int D, int (&ctas_per_sm)[2]);
+struct PagedOccupancy {
+  int ctas_per_sm;
+  int clusters[4];  // resident clusters of 2, 4, 8 and 16 CTAs
+};
+// For the variants with up to 8 and up to 16 heads per unit.
+cudaError_t paged_attn_prepare(bool int8, int D, PagedOccupancy (&occ)[2]);
 cudaError_t launch_paged_attn(const PagedLaunch& a, cudaStream_t stream);
 
 // One call of the paged append (append_paged.cu).

@@ -149,7 +149,8 @@ def test_attention_splits_and_batches(fqkv, int8, lens):
     w0 = w.clone()
     out2 = c.attend(fqkv, q, weights=w)
     c.check(fqkv, q, out2, w0, w)
-    assert torch.equal(out, out2) and torch.equal(out, c.attend(fqkv, q))  # nothing depends on timing
+    # nothing depends on timing (with weights the work may be split in another way: other last bits)
+    assert torch.equal(out, c.attend(fqkv, q)) and torch.equal(out2, c.attend(fqkv, q, weights=w))
     _clean(fqkv)
 
 
