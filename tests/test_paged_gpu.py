@@ -65,6 +65,15 @@ class Cache:
         self.K, self.V = pools
         self.Ks, self.Vs = scales if int8 else (None, None)
 
+    def widen(self):
+        """More columns in the table than clusters take: the plan that puts all tiles in one line."""
+        more = 8192 // self.page + 1
+        junk = torch.randint(-2 ** 31, 2 ** 31 - 1, (self.B, more), generator=torch.Generator().manual_seed(more),
+                             dtype=torch.int64).to(torch.int32).cuda()
+        self.table = torch.cat([self.table, junk], 1).contiguous()
+        self.cap = self.table.shape[1] * self.page
+        return self
+
     def values(self):
         out = []
         for x, s in ((self.K, self.Ks), (self.V, self.Vs)):
@@ -108,6 +117,10 @@ def _clean(fqkv):
     assert fqkv.ops.device_status(torch.device("cuda", 0)) == 0
 
 
+# The two ways the work is split: a thread-block cluster per (sequence, KV head) for small capacities, all tiles in one
+# line otherwise (and always when weights are accumulated).
+PLANS = pytest.mark.parametrize("line", [False, True])
+
 EDGE = [0, 1, 15, 16, 17, 63, 64, 65, 127, 128, 129, 200]
 
 
@@ -115,8 +128,11 @@ EDGE = [0, 1, 15, 16, 17, 63, 64, 65, 127, 128, 129, 200]
 @pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("page", [16, 32, 48, 64, 128, 208])
-def test_attention_edge_lengths(fqkv, int8, D, page):
+@PLANS
+def test_attention_edge_lengths(fqkv, int8, D, page, line):
     c = Cache(fqkv, EDGE, 2, D, page, int8, seed=page)
+    if line:
+        c.widen()
     q = _q(c.B, 8, D)
     c.check(fqkv, q, c.attend(fqkv, q))
     _clean(fqkv)
@@ -133,6 +149,8 @@ def test_attention_head_layouts(fqkv, int8, Hq, Hkv, D):
     out = torch.full((c.B, Hq, D), 7.0, dtype=torch.bfloat16, device="cuda")
     assert c.attend(fqkv, q, out=out, weights=w) is out
     c.check(fqkv, q, out, w0, w)
+    c.check(fqkv, q, c.attend(fqkv, q))
+    c.check(fqkv, q, c.widen().attend(fqkv, q))
     _clean(fqkv)
 
 
@@ -166,7 +184,8 @@ def test_attention_ignores_lengths_past_the_table(fqkv, int8):
     _clean(fqkv)
 
 
-def test_attention_int8_scales_of_every_size(fqkv):
+@PLANS
+def test_attention_int8_scales_of_every_size(fqkv, line):
     """Scales from subnormal to the largest, and zero, in one sequence: small ones keep their precision where
     they are alone, and a later large one rescales what came before."""
     c = Cache(fqkv, [400, 400, 400], 2, 128, 16, True)
@@ -177,6 +196,8 @@ def test_attention_int8_scales_of_every_size(fqkv):
     for i in range(25):  # sequence 1: ascending over its pages; sequence 2: only subnormal and zero scales
         c.Vs[int(c.table[1, i])] = 2.0 ** (i - 20)
         c.Vs[int(c.table[2, i])] = 0.0 if i % 2 else 2.0 ** -23
+    if line:
+        c.widen()
     q = _q(3, 8, 128)
     out = c.attend(fqkv, q)
     K, V = c.values()
@@ -191,11 +212,14 @@ def test_attention_int8_scales_of_every_size(fqkv):
     _clean(fqkv)
 
 
-def test_attention_masked_lowest_and_infinite_values(fqkv):
+@PLANS
+def test_attention_masked_lowest_and_infinite_values(fqkv, line):
     """Rows whose scores reach the fp16 range's ends; an infinite key in an attended slot makes that row NaN only."""
     c = Cache(fqkv, [130, 130], 1, 64, 16, False)
     c.K[int(c.table[0, 2]), 0, 3] = 0
     c.K[int(c.table[0, 2]), 0, 3, 0] = -65504.0
+    if line:
+        c.widen()
     q = _q(2, 4, 64)
     c.check(fqkv, q, c.attend(fqkv, q))
     c.K[int(c.table[0, 2]), 0, 3, 0] = float("nan")
@@ -288,8 +312,11 @@ def test_pool_past_32_bit_offsets(fqkv, int8):
 
 
 @pytest.mark.parametrize("int8", [False, True])
-def test_bad_page_is_reported_and_stays_inside_its_sequence(fqkv, int8):
+@PLANS
+def test_bad_page_is_reported_and_stays_inside_its_sequence(fqkv, int8, line):
     c = Cache(fqkv, [40, 100, 33], 2, 64, 16, int8)
+    if line:
+        c.widen()
     q = _q(3, 8, 64)
     good = c.attend(fqkv, q).clone()
     for bad in (c.P, -1, 2 ** 31 - 1, -2 ** 31):
@@ -305,11 +332,14 @@ def test_bad_page_is_reported_and_stays_inside_its_sequence(fqkv, int8):
     _clean(fqkv)
 
 
-def test_attention_stalled_pipeline_gives_up(fqkv):
+@PLANS
+def test_attention_stalled_pipeline_gives_up(fqkv, line):
     """The failure path of the other decode kernels: tiles that never arrive end the launch with status 61."""
     lib = fqkv.native.lib()
     for int8 in (False, True):
         c = Cache(fqkv, [300, 70], 2, 128, 16, int8)
+        if line:
+            c.widen()
         q = _q(2, 8, 128)
         lib.fqkv_set_wait_timeout_ms(50)
         lib.fqkv_debug_skip_loads(1)
@@ -358,9 +388,33 @@ def test_attention_graph_follows_lengths_and_shares_a_workspace(fqkv, int8):
         for x, o, w in zip((c, d), outs, ws_w):
             x.check(fqkv, q, o, torch.zeros_like(w), w / 2)
     with torch.cuda.stream(side):
-        out = d.attend(fqkv, q)
+        d.attend(fqkv, q, out=outs[0], weights=ws_w[0].new_zeros(ws_w[1].shape))
     side.synchronize()
-    assert torch.equal(out, outs[1])
+    assert torch.equal(outs[0], outs[1])
+    # without weights: the cluster plan, captured, and eager on the other stream
+    with torch.cuda.stream(side):
+        d.attend(fqkv, q, out=outs[1])
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        d.attend(fqkv, q, out=outs[0])
+    for lens in ([64, 1, 500], [0, 1, 480], [3, 0, 0]):
+        d.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        g.replay()
+        torch.cuda.synchronize()
+        d.check(fqkv, q, outs[0])
+    _clean(fqkv)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("lens,Hkv", [([8000], 1), ([3900, 10], 8), ([2000, 1, 0, 700, 2040, 5, 64, 1999], 8), ([120] * 9, 3)])
+def test_attention_clusters_of_every_size(fqkv, int8, lens, Hkv):
+    """Sixteen, eight and four CTAs per unit, with CTAs that get no tile."""
+    c = Cache(fqkv, lens, Hkv, 128, 64, int8, seed=len(lens), extra_pages=0)
+    q = _q(c.B, Hkv * 3, 128, sigma=2.0)
+    out = c.attend(fqkv, q)
+    c.check(fqkv, q, out)
+    assert torch.equal(out, c.attend(fqkv, q))
     _clean(fqkv)
 
 
