@@ -714,6 +714,177 @@ def test_evict_bad_page_is_reported(fqkv):
     _clean(fqkv)
 
 
+# ------------------------------------------------------------------ calls at the edges of what is documented
+@pytest.mark.parametrize("int8", [False, True])
+def test_zero_queries_and_tiny_capacities(fqkv, int8):
+    """q = 0 is the mean over the tokens; a capacity of one tile needs no parts, with weights and without."""
+    c = Cache(fqkv, [16, 3, 0, 1], 2, 64, 16, int8)
+    assert c.cap == 32
+    q = _q(4, 6, 64)
+    q[0] = 0
+    q[1, 2] = 0
+    c.check(fqkv, q, c.attend(fqkv, q))
+    w = torch.rand(4, 2, c.cap, generator=torch.Generator().manual_seed(2)).cuda()
+    w0 = w.clone()
+    c.check(fqkv, q, c.attend(fqkv, q, weights=w), w0, w)
+    c.check(fqkv, q, c.widen().attend(fqkv, q))
+    _clean(fqkv)
+
+
+def test_empty_batches_and_no_tokens(fqkv):
+    K = torch.zeros(2, 1, 16, 64, dtype=torch.float16, device="cuda")
+    none, table = torch.zeros(0, dtype=torch.int32, device="cuda"), torch.zeros(0, 3, dtype=torch.int32, device="cuda")
+    out = fqkv.decode_attn_gqa_paged(K.new_zeros(0, 2, 64), K, K, table, none)
+    assert out.shape == (0, 2, 64)
+    assert fqkv.evict_kvcache_paged(K, K, table, none, torch.zeros(0, 1, 48, device="cuda"), 4, 1).shape == (0,)
+    cos = torch.ones(4, 32, device="cuda")
+    one = torch.zeros(1, 3, dtype=torch.int32, device="cuda")
+    fqkv.rope_qkv_append_paged(K.new_zeros(0, 4 * 64), cos, cos, none, none, one, K.new_zeros(0, 2, 64), K, K)
+    _clean(fqkv)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_two_streams_at_once(fqkv, int8):
+    """Eight calls on two streams, nothing waiting between them, each with its own scratch: the results of calls
+    made alone."""
+    caches = [Cache(fqkv, lens, 2, 64, 16, int8, seed=i) for i, lens in enumerate(([700, 90, 3], [33, 1200, 64]))]
+    caches[1].widen()
+    q = _q(3, 8, 64)
+    alone = [c.attend(fqkv, q).clone() for c in caches]
+    w = [torch.rand(3, 2, c.cap, generator=torch.Generator().manual_seed(4)).cuda() for c in caches]
+    kept = []
+    for c, x in zip(caches, w):  # an eviction made alone, on copies
+        k, v = c.K.clone(), c.V.clone()
+        extra = (None, None) if not int8 else (c.Ks.clone(), c.Vs.clone())
+        fqkv.evict_kvcache_paged(k, v, c.table, c.lens, x.clone(), 50, 9, *extra)
+        kept.append((k, v))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                outs[i].append(caches[i].attend(fqkv, q))
+    for i, st in enumerate(streams):
+        with torch.cuda.stream(st):
+            fqkv.evict_kvcache_paged(caches[i].K, caches[i].V, caches[i].table, caches[i].lens, w[i], 50, 9, caches[i].Ks,
+                                     caches[i].Vs)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, alone[i]) for o in outs[i])
+        for a, b in zip((caches[i].K, caches[i].V), kept[i]):
+            dt = torch.int8 if int8 else torch.int16
+            assert torch.equal(a.contiguous().view(dt), b.contiguous().view(dt))
+    _clean(fqkv)
+
+
+def test_sliced_positions_and_tables(fqkv):
+    """Rows of wider tensors for positions, the table and the pools, in the append and the eviction."""
+    D, Hq, Hkv, page, B = 64, 4, 2, 16, 3
+    g = torch.Generator().manual_seed(3)
+    big = torch.zeros(2, 12, Hkv, page, D, dtype=torch.float16, device="cuda")
+    K, V = big[0, 1:], big[1, 1:]
+    wide = torch.full((B, 9), -5, dtype=torch.int32, device="cuda")
+    wide[:, 4:6] = torch.tensor([[3, 7], [0, 5], [9, 2]], dtype=torch.int32)
+    table = wide[:, 4:7]
+    cos, sin = _tables(64, D)
+    T = 3 * 20
+    pos_wide = torch.randint(64, (5, T + 13), generator=g, dtype=torch.int32).cuda()
+    pos = pos_wide[1:3, 6:6 + T]
+    seqs = (torch.arange(T, dtype=torch.int32) // 20).cuda()
+    slots = (torch.arange(T, dtype=torch.int32) % 20).cuda()
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * D, generator=g).half().cuda()
+    axes = fqkv.rope_axes([20, 12])
+    q1, q2 = (torch.empty(T, Hq, D, dtype=torch.float16, device="cuda") for _ in range(2))
+    fqkv.rope_qkv_append_paged(qkv, cos, sin, pos, slots, table, q1, K, V, axes=axes, seq_ids=seqs)
+    K2, V2 = torch.zeros_like(K).contiguous(), torch.zeros_like(V).contiguous()
+    fqkv.rope_qkv_append_paged(qkv, cos, sin, pos.contiguous(), slots, table.contiguous(), q2, K2, V2, axes=axes, seq_ids=seqs)
+    assert torch.equal(q1, q2) and torch.equal(K, K2) and torch.equal(V, V2) and float(K2.abs().sum()) > 0
+    assert float(big[:, 0].abs().sum()) == 0
+    lens = torch.full((B,), 20, dtype=torch.int32, device="cuda")
+    w = torch.rand(B, Hkv, 3 * page, generator=g).cuda()
+    a = fqkv.evict_kvcache_paged(K, V, table, lens, w.clone(), 9, 4)
+    b = fqkv.evict_kvcache_paged(K2, V2, table.contiguous(), lens, w.clone(), 9, 4)
+    assert torch.equal(a, b) and torch.equal(K, K2) and torch.equal(V, V2)
+    _clean(fqkv)
+
+
+def test_refusals_of_the_python_layer(fqkv):
+    c = Cache(fqkv, [20, 5], 2, 64, 16, False)
+    i8 = Cache(fqkv, [20, 5], 2, 64, 16, True)
+    q = _q(2, 4, 64)
+    w = torch.zeros(2, 2, c.cap, device="cuda")
+
+    def attn(match, **kw):
+        a = dict(q=q, K=c.K, V=c.V, block_table=c.table, seq_lens=c.lens)
+        a.update(kw)
+        with pytest.raises(RuntimeError, match=match):
+            fqkv.decode_attn_gqa_paged(**a)
+
+    attn("^fp16", q=q.float())
+    attn("^fp16", q=q.transpose(1, 2).contiguous().transpose(1, 2))
+    attn("^shape", q=q[:1])
+    attn("^shape", V=c.V[:1])
+    attn("^fp16", K=i8.K, V=i8.V)
+    attn("^stride", K=c.K.transpose(2, 3).contiguous().transpose(2, 3))
+    attn("^D", K=c.K[..., :32], V=c.V[..., :32], q=q[..., :32].contiguous())
+    attn("^block_table", block_table=c.table.long())
+    attn("^seq_lens", seq_lens=c.lens.long())
+    attn("^seq_lens", seq_lens=c.lens[:1])
+    attn("^cuda", seq_lens=c.lens.cpu())
+    attn("^weights", weights=w[:, :1])
+    attn("^weights", weights=w.half())
+    attn("^dtype", out=torch.empty(2, 4, 64, device="cuda"))
+    attn("^shape", out=torch.empty(2, 4, 32, dtype=torch.float16, device="cuda"))
+    attn("^workspace", workspace=torch.empty(1000, dtype=torch.uint8))
+    attn("needed", workspace=torch.empty(16, dtype=torch.uint8, device="cuda"), weights=w)
+    attn("multiple of 16", K=c.K[:, :, :8], V=c.V[:, :, :8])
+    attn("multiple of Hkv", q=_q(2, 3, 64))
+    with pytest.raises(RuntimeError, match="^fp16"):
+        fqkv.decode_attn_gqa_int8_paged(q, i8.K, i8.V, i8.Ks, None, i8.table, i8.lens)
+    with pytest.raises(RuntimeError, match="^shape"):
+        fqkv.decode_attn_gqa_int8_paged(q, i8.K, i8.V, i8.Ks[:1], i8.Vs, i8.table, i8.lens)
+
+    def evict(match, **kw):
+        a = dict(K=c.K, V=c.V, block_table=c.table, seq_lens=c.lens, weights=w, budget=4, recent=1)
+        a.update(kw)
+        with pytest.raises(RuntimeError, match=match):
+            fqkv.evict_kvcache_paged(**a)
+
+    evict("budget", budget=0)
+    evict("recent", recent=5)
+    evict("^weights", weights=w[:, :, :-1])
+    evict("^weights_out", weights_out=w.double())
+    evict("^lens_out", lens_out=c.lens[:1])
+    evict("^fp16", Ks=i8.Ks)
+    evict("needed", workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    both = torch.zeros(w.numel() + 16, device="cuda")
+    evict("overlap", weights=both[:w.numel()].view(w.shape), weights_out=both[16:].view(w.shape))
+
+    cos = torch.ones(8, 32, device="cuda")
+    qkv = torch.zeros(2, 8 * 64, dtype=torch.float16, device="cuda")
+    i = torch.zeros(2, dtype=torch.int32, device="cuda")
+
+    def append(match, **kw):
+        a = dict(qkv=qkv, cos_table=cos, sin_table=cos, positions=i, slots=i, block_table=c.table, q_out=q.clone(), K=c.K, V=c.V)
+        a.update(kw)
+        with pytest.raises(RuntimeError, match=match):
+            fqkv.rope_qkv_append_paged(**a)
+
+    append("^dtype", qkv=qkv.float())
+    append("^shape", qkv=qkv[:, :-64])
+    append("^shape", qkv=qkv[:1])
+    append("^tables", cos_table=cos.half())
+    append("^tables", sin_table=cos[:, :16])
+    append("^positions", positions=i[:1])
+    append("^axes", positions=torch.stack([i, i]))
+    append("^axes", positions=torch.stack([i, i]), axes=i)
+    append("^slots", slots=i.long())
+    append("^seq_ids", seq_ids=i[:1])
+    append("aligned", qkv=torch.zeros(2, 8 * 64 + 4, dtype=torch.float16, device="cuda")[:, 4:])
+    _clean(fqkv)
+
+
 # ------------------------------------------------------------------ together
 @pytest.mark.parametrize("int8", [False, True])
 def test_decode_loop_with_eviction(fqkv, int8):
