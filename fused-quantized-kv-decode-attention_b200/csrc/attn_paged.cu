@@ -788,7 +788,8 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
     const int S = a.cluster, r = int(cluster_ctarank());
     const int gvalid = min(a.GP, a.G - (walk.u % a.groups) * a.GP);
     const size_t row_base = size_t(walk.b) * a.Hq + size_t(walk.u / a.groups) * a.G + size_t(walk.u % a.groups) * a.GP;
-    if (walk.end == 0 && ct < gvalid) *reinterpret_cast<float2*>(cl_ml + 2 * ct) = make_float2(-INFINITY, 0.f);  // no tiles
+    // a CTA without tiles has the sum -1, which no other can have; its outputs are never written
+    if (walk.end == 0 && ct < gvalid) *reinterpret_cast<float2*>(cl_ml + 2 * ct) = make_float2(-INFINITY, -1.f);
     cluster_sync_all();
     // the outputs, two dimensions at a time, shared out over the cluster; parts always in CTA order
     for (int i = r * (32 * kWarps) + ct; i < gvalid * (D / 2); i += S * 32 * kWarps) {
@@ -798,7 +799,7 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
       float M = -INFINITY;
 #pragma unroll
       for (int j = 0; j < kMaxCluster; ++j) {
-        ml[j] = make_float2(-INFINITY, 0.f);
+        ml[j] = make_float2(-INFINITY, -1.f);
         o[j] = make_float2(0.f, 0.f);
         if (j < S) {
           ml[j] = ld_dsmem_f32x2(dsmem_addr(ml_at, j));
@@ -810,8 +811,7 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
       float2 O = make_float2(0.f, 0.f);
 #pragma unroll
       for (int j = 0; j < kMaxCluster; ++j) {
-        // no say: a CTA without tiles (its o was never written); sums of NaN scores have maximum -inf and stay
-        if (ml[j].x == -INFINITY && ml[j].y == 0.f) continue;
+        if (ml[j].y == -1.f) continue;
         const float w = M == -INFINITY ? 1.f : ex2(ml[j].x - M);
         L += w * ml[j].y;
         O.x += w * o[j].x;

@@ -1005,16 +1005,16 @@ static int paged_heads(int64_t Hq, const fqkv::PagedCache& c) {
   if (Hq < 1 || Hq % c.Hkv != 0)
     return fail(FQKV_ERR_INVALID_ARGUMENT, "Hq (%lld) must be a multiple of Hkv (%d)", (long long)Hq, c.Hkv);
   if (Hq > 65535 || int64_t(c.B) * Hq > INT32_MAX) return fail(FQKV_ERR_INVALID_ARGUMENT, "sizes exceed the index range");
-  // the tiles of all units are numbered in 32 bits
+  // the tiles of all units are numbered in 32 bits, with room for a CTA's share past the last one
   const int64_t groups = (Hq / c.Hkv + fqkv::kPagedMaxHeads - 1) / fqkv::kPagedMaxHeads;
-  if (int64_t(c.B) * c.Hkv * groups * (int64_t(c.cap) / 64 + 1) > INT32_MAX)
+  if (int64_t(c.B) * c.Hkv * groups * (int64_t(c.cap) / 64 + 1) > INT32_MAX / 2)
     return fail(FQKV_ERR_INVALID_ARGUMENT, "sizes exceed the index range");
   return FQKV_OK;
 }
 
 size_t fqkv_paged_workspace_bytes(int kv_format, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len, int weights) {
   if ((kv_format != FQKV_KV_F16 && kv_format != FQKV_KV_INT8) || B < 1 || B > 65535 || Hkv < 1 || Hkv > 65535 || Hq < 1 ||
-      Hq > 65535 || Hq % Hkv != 0 || (D != 64 && D != 128) || max_len < 1 || max_len > INT32_MAX)
+      Hq > 65535 || Hq % Hkv != 0 || (D != 64 && D != 128) || max_len < 1 || max_len > (int64_t(1) << 30))
     return 0;
   DeviceState* ds = nullptr;
   if (device_state(&ds) != FQKV_OK) return 0;
@@ -1125,7 +1125,7 @@ int fqkv_rope_append_paged(const fqkv_paged_kv_t* kv, int32_t model_dtype, const
                 (long long)kv->B);
   if (qkv_row_stride < (Hq + 2 * kv->Hkv) * kv->D)
     return fail(FQKV_ERR_INVALID_ARGUMENT, "qkv_row_stride %lld < (Hq + 2 Hkv) D", (long long)qkv_row_stride);
-  if (axes > 1 && position_stride < T)
+  if (axes > 1 && position_stride != 0 && position_stride < T)
     return fail(FQKV_ERR_INVALID_ARGUMENT, "positions: row stride %lld < T", (long long)position_stride);
   if (!qkv || !cos_table || !sin_table || !positions || !slots || !q_out || (axes > 1 && !axis_map))
     return fail(FQKV_ERR_INVALID_ARGUMENT, "null tensor pointer");
@@ -1133,6 +1133,7 @@ int fqkv_rope_append_paged(const fqkv_paged_kv_t* kv, int32_t model_dtype, const
     return fail(FQKV_ERR_MISALIGNED, "qkv rows, tables and q_out must be 16-byte aligned");
   if (!aligned(positions, 4) || !aligned(slots, 4) || (seq_ids && !aligned(seq_ids, 4)) || (axis_map && !aligned(axis_map, 4)))
     return fail(FQKV_ERR_MISALIGNED, "positions, slots, seq_ids and axis_map must be 4-byte aligned");
+  if (kv->k == kv->v) return fail(FQKV_ERR_INVALID_ARGUMENT, "kv: K and V must be different pools to be written");
   DeviceState* ds = nullptr;
   if (int rc = device_state(&ds)) return rc;
   a.qkv = qkv; a.qkv_stride = qkv_row_stride;
@@ -1154,7 +1155,7 @@ int fqkv_rope_append_paged(const fqkv_paged_kv_t* kv, int32_t model_dtype, const
 }
 
 size_t fqkv_evict_workspace_bytes(int64_t B, int64_t Hkv, int64_t max_len, int64_t budget) {
-  if (B < 1 || Hkv < 1 || B > 65535 || Hkv > 65535 || max_len < 1 || budget < 1) return 0;
+  if (B < 1 || Hkv < 1 || B > 65535 || Hkv > 65535 || max_len < 1 || max_len > (int64_t(1) << 30) || budget < 1) return 0;
   const size_t units = size_t(B) * size_t(Hkv);
   return pad256(units * sizeof(int2)) + pad256(units * size_t(std::min(max_len, budget)) * sizeof(int));
 }
@@ -1181,6 +1182,7 @@ int fqkv_evict_paged(const fqkv_paged_kv_t* kv, const float* weights, float* wei
     return fail(FQKV_ERR_INVALID_ARGUMENT, "workspace: %zu bytes given, %zu needed", workspace ? workspace_bytes : size_t(0),
                 need);
   if (!aligned(workspace, 16)) return fail(FQKV_ERR_MISALIGNED, "workspace must be 16-byte aligned");
+  if (kv->k == kv->v) return fail(FQKV_ERR_INVALID_ARGUMENT, "kv: K and V must be different pools to be written");
   DeviceState* ds = nullptr;
   if (int rc = device_state(&ds)) return rc;
   a.weights = weights; a.weights_out = weights_out;

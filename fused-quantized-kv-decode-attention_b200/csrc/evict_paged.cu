@@ -18,8 +18,9 @@
 // head), chunk by chunk in list order; a chunk is written only after it and all earlier chunks were read, and a
 // chunk's writes end below the next chunk's first source, so reading ahead is free.  Slices make enough CTAs for
 // few sequences.  The chunks before the first gap are not touched.  Two chunks of 32 KB in flight in each of three CTAs
-// per SM (three in each of two: 97 us instead of 95 us for 16 sequences; 16 KB chunks: 99 to 135 us).  (One launch, with a cluster per (sequence, KV head) that
-// selects and then moves, was 5 us slower for one sequence -- a cluster's barriers -- and no faster for many.)
+// per SM (three in each of two: 97 us instead of 95 us for 16 sequences; 16 KB chunks: 99 to 135 us).  (One launch,
+// with a cluster per (sequence, KV head) that selects and then moves, was 5 us slower for one sequence -- a cluster's
+// barriers -- and no faster for many.)
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 

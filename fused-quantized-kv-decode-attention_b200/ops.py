@@ -891,8 +891,7 @@ def _workspace_size(idx: int, fn, *args) -> int:
         n = int(_on_gpu(idx, getattr(_native.lib(), fn), *args))
         if len(_workspace_sizes) >= 1024:
             _workspace_sizes.clear()
-        if n:  # 0: refused, the call itself says why
-            _workspace_sizes[key] = n
+        _workspace_sizes[key] = n  # 0: none needed, or refused (the call says why and forgets it)
     return n
 
 
@@ -937,6 +936,7 @@ def _decode_paged(op, q, K, V, Ks, Vs, block_table, seq_lens, out, workspace, we
     rc = _on_gpu(idx, _native.lib().fqkv_decode_attn_paged, desc, bf16, q.data_ptr(), out.data_ptr(), Hq, w, ws, nb,
                  _stream_of(idx))
     if rc:
+        _workspace_sizes.clear()
         _native.check(rc, f"launch: {op}")
     return out
 
@@ -995,12 +995,13 @@ def rope_qkv_append_paged(qkv: torch.Tensor, cos_table: torch.Tensor, sin_table:
 
     qkv [T,W] (fp16 or bf16, rows 16-byte aligned) holds [q heads | k heads | v heads]; cos_table / sin_table
     [rows,D/2] float32, one column per rotary pair (i, i + D/2).  ``positions`` int32: [T], or [A,T] with ``axes``
-    (int32 [D/2], see :func:`rope_axes`) saying which row each pair turns with.  Token t goes to slot ``slots[t]``
+    (int32 [D/2], see :func:`rope_axes`) saying which row each pair turns with (``pos.expand(A, T)`` is fine).  Token t goes to slot ``slots[t]``
     of sequence ``seq_ids[t]`` (None: sequence t); a negative slot is padding and nothing of the token is written.
     A position need not equal the slot (after an eviction it does not).  q_out [T,Hq,D] fp16; K/V and Ks/Vs as in
     :func:`decode_attn_gqa_paged` / :func:`decode_attn_gqa_int8_paged`; int8 codes and scales are :func:`qpt`'s of the
     fp16 row.  fp32 arithmetic, rounded once.  A token out of range is not written and reported by
-    :func:`check_device_status`; two tokens of one call must not share a slot.
+    :func:`check_device_status`; two tokens of one call must not share a slot,
+    and q_out must not overlap qkv.
     """
     op = "rope_qkv_append_paged"
     ts = (qkv, cos_table, sin_table, positions, slots, block_table, q_out, K, V) + _scales(op, Ks, Vs)
@@ -1078,7 +1079,11 @@ def evict_kvcache_paged(K: torch.Tensor, V: torch.Tensor, block_table: torch.Ten
         lens_out = torch.empty_like(seq_lens)
     else:
         _index_vector(op, "lens_out", lens_out, B)
-    budget = int(budget)
+    budget, recent = int(budget), int(recent)
+    if not 0 <= recent <= budget:
+        _fail(op, "recent", f"recent must be in [0, budget = {budget}] (got {recent})")
+    if budget > cap:  # evicts nothing; a C integer may not hold it
+        budget, recent = cap, min(recent, cap)
     if workspace is None:
         nb = _workspace_size(idx, "fqkv_evict_workspace_bytes", B, Hkv, cap, budget) if B else 0
         workspace = torch.empty(nb, dtype=torch.uint8, device=K.device) if nb else None
@@ -1086,7 +1091,8 @@ def evict_kvcache_paged(K: torch.Tensor, V: torch.Tensor, block_table: torch.Ten
     else:
         ws, nb = _scratch(op, workspace, idx)
     rc = _on_gpu(idx, _native.lib().fqkv_evict_paged, desc, weights.data_ptr(), weights_out.data_ptr(), lens_out.data_ptr(),
-                 budget, int(recent), ws, nb, _stream_of(idx))
+                 budget, recent, ws, nb, _stream_of(idx))
     if rc:
+        _workspace_sizes.clear()
         _native.check(rc, f"launch: {op}")
     return lens_out

@@ -393,7 +393,8 @@ size_t fqkv_paged_workspace_bytes(int kv_format, int64_t B, int64_t Hq, int64_t 
  * fp32, rounded once to f16.  A token with a negative slot is padding:
  * nothing of it is written, q_out included.  One whose sequence, slot, axes or
  * positions are out of range is not written either and records status 66 (65:
- * its page).  Two tokens of one call must not share a slot.  seq_lens is not used.  Extends
+ * its page).  Two tokens of one call must not share a slot, and q_out must not
+ * overlap qkv.  position_stride is 0 (one row for all axes) or at least T.  seq_lens is not used.  Extends
  * fqkv_rope_qkv_append, whose rounding follows transformers' in the model dtype. */
 int fqkv_rope_append_paged(const fqkv_paged_kv_t* kv, int32_t model_dtype, const void* qkv, int64_t qkv_row_stride,
                            const float* cos_table, const float* sin_table, int64_t table_rows, const int32_t* positions,

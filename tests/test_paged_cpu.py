@@ -134,6 +134,25 @@ def test_evict_arguments_rejected(fqkv):
         assert rc == code and word in msg, (kw, rc, msg)
 
 
+def test_one_pool_for_keys_and_values_is_not_written(fqkv):
+    """Reading it is fine; an append or an eviction would write one over the other."""
+    lib = fqkv.native.lib()
+    need = lib.fqkv_evict_workspace_bytes(2, 2, 64, 8)
+    assert lib.fqkv_evict_paged(_kv(fqkv), A16, A16, A16, 8, 2, A16, need, None) == BAD
+    assert "different pools" in fqkv.native.last_error()
+    assert lib.fqkv_rope_append_paged(_kv(fqkv), 0, A16, 8 * 64, A16, A16, 10, A16, 2, 1, None, None, A16, A16, 2, 4, None) == BAD
+    assert "different pools" in fqkv.native.last_error()
+
+
+def test_sizes_past_the_index_range_have_no_workspace(fqkv):
+    lib = fqkv.native.lib()
+    assert lib.fqkv_paged_workspace_bytes(0, 1, 1, 1, 64, 2 ** 30 + 16, 1) == 0
+    assert lib.fqkv_evict_workspace_bytes(1, 1, 2 ** 30 + 16, 2 ** 40) == 0
+    # 16384 x 4 heads in groups of 16, of 2^30 tokens: the tiles have no 32-bit numbers
+    rc, msg = _attn(fqkv, _kv(fqkv, B=16384, Hkv=4, max_pages=2 ** 26, table_stride=2 ** 26), Hq=4 * 17)
+    assert rc == BAD and "index range" in msg
+
+
 def test_python_layer_refuses_cpu_tensors(fqkv):
     K = torch.zeros(2, 1, 16, 64, dtype=torch.float16)
     i = torch.zeros(1, 2, dtype=torch.int32)

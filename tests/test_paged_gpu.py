@@ -851,7 +851,9 @@ def test_refusals_of_the_python_layer(fqkv):
         with pytest.raises(RuntimeError, match=match):
             fqkv.evict_kvcache_paged(**a)
 
-    evict("budget", budget=0)
+    evict("budget", budget=0, recent=0)
+    evict("budget", budget=-3, recent=-3)
+    evict("recent", budget=0)
     evict("recent", recent=5)
     evict("^weights", weights=w[:, :, :-1])
     evict("^weights_out", weights_out=w.double())
@@ -882,6 +884,53 @@ def test_refusals_of_the_python_layer(fqkv):
     append("^slots", slots=i.long())
     append("^seq_ids", seq_ids=i[:1])
     append("aligned", qkv=torch.zeros(2, 8 * 64 + 4, dtype=torch.float16, device="cuda")[:, 4:])
+    _clean(fqkv)
+
+
+def test_one_position_row_for_all_axes(fqkv):
+    """Text tokens: the same position on every axis, as an expanded view; as one axis."""
+    D, Hq, Hkv, T = 128, 4, 1, 5
+    g = torch.Generator().manual_seed(8)
+    cos, sin = _tables(64, D)
+    K, V, K2, V2 = (torch.zeros(T, Hkv, 16, D, dtype=torch.float16, device="cuda") for _ in range(4))
+    table = torch.arange(T, dtype=torch.int32, device="cuda")[:, None]
+    pos = torch.randint(64, (T,), generator=g, dtype=torch.int32).cuda()
+    slots = torch.arange(T, dtype=torch.int32, device="cuda")
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * D, generator=g).to(torch.bfloat16).cuda()
+    q1, q2 = (torch.empty(T, Hq, D, dtype=torch.float16, device="cuda") for _ in range(2))
+    fqkv.rope_qkv_append_paged(qkv, cos, sin, pos.expand(3, T), slots, table, q1, K, V, axes=fqkv.rope_axes([20, 22, 22]))
+    fqkv.rope_qkv_append_paged(qkv, cos, sin, pos, slots, table, q2, K2, V2)
+    assert torch.equal(q1, q2) and torch.equal(K, K2) and torch.equal(V, V2) and float(K.abs().sum()) > 0
+    _clean(fqkv)
+
+
+def test_a_budget_past_every_integer_evicts_nothing(fqkv):
+    c = Cache(fqkv, [20, 5], 2, 64, 16, False)
+    w = torch.rand(2, 2, c.cap, device="cuda")
+    k, w0 = c.K.clone(), w.clone()
+    assert fqkv.evict_kvcache_paged(c.K, c.V, c.table, c.lens, w, 2 ** 64 + 1, 2 ** 64).tolist() == [20, 5]
+    assert torch.equal(c.K.view(torch.int16), k.view(torch.int16)) and torch.equal(w, w0)
+    _clean(fqkv)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_a_zero_probability_times_an_infinite_value(fqkv, wide):
+    """A key of score -inf in one tile whose value is inf: 0 * inf is NaN in both plans, as in the definition."""
+    B, D, page = 1, 64, 16
+    K = torch.zeros(40, 1, page, D, dtype=torch.float16, device="cuda")
+    V = torch.ones(40, 1, page, D, dtype=torch.float16, device="cuda")
+    q = torch.zeros(B, 2, D, dtype=torch.float16, device="cuda")
+    q[:, :, 0] = 1
+    K[:4, :, :, 0] = float("-inf")  # the whole first tile of 64 keys
+    V[1, 0, 3, 7] = float("inf")
+    table = torch.arange(40, dtype=torch.int32, device="cuda")[None]
+    if wide:
+        table = torch.cat([table, table.new_zeros(1, 1000)], 1).contiguous()
+    out = fqkv.decode_attn_gqa_paged(q, K, V, table, torch.tensor([640], dtype=torch.int32, device="cuda"))
+    assert bool(out[:, :, 7].isnan().all())
+    rest = torch.ones(D, dtype=torch.bool, device="cuda")
+    rest[7] = False
+    assert torch.equal(out[:, :, rest], torch.ones_like(out[:, :, rest]))
     _clean(fqkv)
 
 
