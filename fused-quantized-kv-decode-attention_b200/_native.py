@@ -43,8 +43,7 @@ class TpOut(ctypes.Structure):
 
 # fqkv_paged_kv_t, packed (no padding): format and a reserved word; page_size, num_pages, max_pages, B, Hkv, D;
 # the K, V, K-scale and V-scale pointers; K and V strides (page, head, token), K-scale and V-scale strides (page,
-# head); block table, its row stride, lengths.  One pack call, where filling a ctypes Structure field by field would
-# cost a decode step several microseconds.
+# head); block table, its row stride, lengths.
 PAGED_KV = struct.Struct("=ii6q4Q6q4qQqQ")
 
 
@@ -108,6 +107,7 @@ class NativeLibraryError(RuntimeError):
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
+_binding = None
 
 
 def lib() -> ctypes.CDLL:
@@ -130,6 +130,26 @@ def lib() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = handle
     return _lib
+
+
+def binding():
+    """The extension module of the paged-cache operators (``csrc/torch_binding.cpp``), bound to the loaded library."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    handle = lib()
+    with _lock:
+        if _binding is None:
+            try:
+                from . import _torch_binding as mod
+            except ImportError as exc:
+                raise NativeLibraryError(
+                    f"_torch_binding.so is not built for this torch ({exc}); run build.py in {LIB_PATH.parent}") from exc
+            mod.bind(*(ctypes.cast(getattr(handle, f), ctypes.c_void_p).value
+                       for f in ("fqkv_last_error", "fqkv_decode_attn_paged", "fqkv_paged_workspace_bytes",
+                                 "fqkv_rope_append_paged", "fqkv_evict_paged", "fqkv_evict_workspace_bytes")))
+            _binding = mod
+    return _binding
 
 
 def last_error() -> str:

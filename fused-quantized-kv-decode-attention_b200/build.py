@@ -6,8 +6,9 @@ Each ``csrc/*.cu`` is compiled to an object in ``_build/`` (in parallel), then
 linked into ``libfqkv_b200.so`` next to this file with the CUDA runtime linked
 statically, so the library depends only on the NVIDIA driver.  ``-Xptxas -v``
 register / spill / shared-memory reports are written to
-``_build/ptxas_<name>.log``.  Rebuilds only when a source or header is newer
-than the library (or with ``--force``).
+``_build/ptxas_<name>.log``.  ``csrc/torch_binding.cpp`` becomes the extension
+module ``_torch_binding.so`` (g++, the installed torch's headers).  Rebuilds
+only when a source or header is newer than the libraries (or with ``--force``).
 """
 from __future__ import annotations
 
@@ -18,12 +19,14 @@ import pathlib
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = pathlib.Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 INCLUDE = HERE.parent / "include"
 BUILD = HERE / "_build"
 LIB = HERE / "libfqkv_b200.so"
+BINDING = HERE / "_torch_binding.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
@@ -44,9 +47,9 @@ def sources() -> list[pathlib.Path]:
 
 
 def _stale() -> bool:
-    if not LIB.exists():
+    if not LIB.exists() or not BINDING.exists():
         return True
-    t = LIB.stat().st_mtime
+    t = min(LIB.stat().st_mtime, BINDING.stat().st_mtime)
     deps = list(CSRC.glob("*")) + list(INCLUDE.glob("*.h")) + [pathlib.Path(__file__)]
     return any(p.stat().st_mtime > t for p in deps)
 
@@ -63,13 +66,36 @@ def _compile(src: pathlib.Path, verbose: bool) -> pathlib.Path:
     return obj
 
 
+def _build_binding(verbose: bool) -> None:
+    """The Python layer of the paged-cache operators, against the torch of this interpreter."""
+    import torch
+
+    root = pathlib.Path(torch.__file__).resolve().parent
+    cuda = pathlib.Path(nvcc()).resolve().parents[1] / "include"
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", str(root / "include"),
+           "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"), "-isystem", str(cuda),
+           str(CSRC / "torch_binding.cpp"), "-o", str(tmp),
+           f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed for torch_binding.cpp:\n{r.stderr[-6000:]}")
+    os.replace(tmp, BINDING)
+    if verbose:
+        print(f"built {BINDING}")
+
+
 def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
     if not force and not _stale():
         return LIB
     BUILD.mkdir(exist_ok=True)
     srcs = sources()
-    with cf.ThreadPoolExecutor(max_workers=min(len(srcs), os.cpu_count() or 4)) as ex:
+    with cf.ThreadPoolExecutor(max_workers=min(len(srcs) + 1, os.cpu_count() or 4)) as ex:
+        binding = ex.submit(_build_binding, verbose)
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
+        binding.result()
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", str(tmp), *map(str, objs)]
     r = subprocess.run(cmd, capture_output=True, text=True)

@@ -782,119 +782,7 @@ def quant_int4_per_token(X: torch.Tensor):
 
 
 # ------------------------------------------------------------------ paged KV cache
-# A decode step calls these every layer, so their checks are written for host time: device numbers instead of device
-# objects, no keyword dictionaries, messages built only when something is wrong.
-_I32, _F16, _F32, _BF16, _I8 = torch.int32, torch.float16, torch.float32, torch.bfloat16, torch.int8
-
-
-def _gpu_of(op: str, *ts) -> int:
-    """The number of the GPU that holds all of ts."""
-    try:
-        idx = ts[0].get_device()
-        for t in ts:
-            if t.get_device() != idx:
-                _fail(op, "cuda", "all tensors must be on the same device")
-    except AttributeError:
-        _fail(op, "cuda", "all tensors must be CUDA tensors (there is no CPU path)")
-    if idx < 0:
-        _fail(op, "cuda", "all tensors must be CUDA tensors (there is no CPU path)")
-    return idx
-
-
-def _on_gpu(idx: int, fn, *args):
-    """fn(*args) with GPU idx current."""
-    if torch.cuda.current_device() == idx:
-        return fn(*args)
-    with torch.cuda.device(idx):
-        return fn(*args)
-
-
-def _stream_of(idx: int) -> int:
-    return _raw_stream(idx) if _raw_stream is not None else torch.cuda.current_stream(idx).cuda_stream
-
-
-def _index_vector(op: str, name: str, t: torch.Tensor, n: int) -> None:
-    if t.dtype is not _I32 or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
-        _fail(op, name, f"{name} must be a contiguous int32 tensor of {n} (got {t.dtype} {tuple(t.shape)})")
-
-
-def _paged_kv(op: str, K, V, Ks, Vs, block_table, seq_lens):
-    """Checks a paged cache (tensors of one GPU); returns (packed descriptor, B, Hkv, D, tokens a sequence can hold)."""
-    shape = K.shape
-    if len(shape) != 4 or V.shape != shape:
-        _fail(op, "shape", "K and V must both be [num_pages, Hkv, page_size, D]")
-    code = _F16 if Ks is None else _I8
-    if K.dtype is not code or V.dtype is not code:
-        _fail(op, "fp16" if Ks is None else "int8", f"K and V must be {code} (got {K.dtype}, {V.dtype})")
-    P, Hkv, page, D = shape
-    k0, k1, k2, k3 = K.stride()
-    v0, v1, v2, v3 = V.stride()
-    if D != 64 and D != 128:
-        _fail(op, "D", f"head_dim must be 64 or 128 (got {D})")
-    if k3 != 1 or v3 != 1:
-        _fail(op, "stride", "K and V must be contiguous over D")
-    tshape = block_table.shape
-    if len(tshape) != 2 or block_table.dtype is not _I32:
-        _fail(op, "block_table", "block_table must be an int32 [B, max_pages] tensor")
-    B, max_pages = tshape
-    t0, t1 = block_table.stride()
-    if t1 != 1 and max_pages > 1:
-        _fail(op, "block_table", "block_table must have contiguous rows")
-    lens = 0
-    if seq_lens is not None:
-        _index_vector(op, "seq_lens", seq_lens, B)
-        lens = seq_lens.data_ptr()
-    ks = vs = ks0 = ks1 = vs0 = vs1 = fmt = 0
-    if Ks is not None:
-        fmt = _native.KV_INT8
-        if Ks.dtype is not _F16 or Vs.dtype is not _F16:
-            _fail(op, "fp16", f"Ks and Vs must be {_F16} (got {Ks.dtype}, {Vs.dtype})")
-        if Ks.shape != (P, Hkv, page) or Vs.shape != (P, Hkv, page):
-            _fail(op, "shape", f"Ks and Vs must be [num_pages, Hkv, page_size] = {(P, Hkv, page)}")
-        ks0, ks1, ks2 = Ks.stride()
-        vs0, vs1, vs2 = Vs.stride()
-        if ks2 != 1 or vs2 != 1:
-            _fail(op, "stride", "Ks and Vs must be contiguous over a page's tokens")
-        ks, vs = Ks.data_ptr(), Vs.data_ptr()
-    desc = _native.PAGED_KV.pack(fmt, 0, page, P, max_pages, B, Hkv, D, K.data_ptr(), V.data_ptr(), ks, vs, k0, k1, k2, v0,
-                                 v1, v2, ks0, ks1, vs0, vs1, block_table.data_ptr(), t0, lens)
-    return desc, B, Hkv, D, max_pages * page
-
-
-def _scales(op: str, Ks, Vs) -> tuple:
-    """The scale tensors among a call's inputs: none or both."""
-    if (Ks is None) != (Vs is None):
-        _fail(op, "fp16", "Ks and Vs go together")
-    return () if Ks is None else (Ks, Vs)
-
-
-def _scratch(op: str, workspace: torch.Tensor, idx: int):
-    """(pointer, bytes) of the caller's workspace."""
-    if not isinstance(workspace, torch.Tensor) or workspace.get_device() != idx or not workspace.is_contiguous():
-        _fail(op, "workspace", "workspace must be a contiguous tensor on the inputs' device")
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
-
-
-def _slot_weights(op: str, name: str, w, shape) -> None:
-    if w.dtype is not _F32 or w.shape != shape or not w.is_contiguous():
-        _fail(op, name, f"{name} must be a contiguous float32 {list(shape)} tensor (got {w.dtype} {tuple(w.shape)})")
-
-
-# Workspace sizes by (GPU, arguments): they depend on nothing else.
-_workspace_sizes: dict = {}
-
-
-def _workspace_size(idx: int, fn, *args) -> int:
-    key = (idx, fn, *args)
-    n = _workspace_sizes.get(key)
-    if n is None:
-        n = int(_on_gpu(idx, getattr(_native.lib(), fn), *args))
-        if len(_workspace_sizes) >= 1024:
-            _workspace_sizes.clear()
-        _workspace_sizes[key] = n  # 0: none needed, or refused (the call says why and forgets it)
-    return n
-
-
+# A decode step calls these every layer: their checks and launches are compiled (csrc/torch_binding.cpp).
 def paged_workspace_bytes(kv_format: str, B: int, Hq: int, Hkv: int, max_len: int, D: int, weights: bool = False) -> int:
     """Workspace of a paged decode call on the current device; max_len = max_pages * page_size."""
     fmt = {"fp16": _native.KV_F16, "int8": _native.KV_INT8}[kv_format]
@@ -904,41 +792,6 @@ def paged_workspace_bytes(kv_format: str, B: int, Hq: int, Hkv: int, max_len: in
 def evict_workspace_bytes(B: int, Hkv: int, max_len: int, budget: int) -> int:
     """Workspace of :func:`evict_kvcache_paged`; max_len = max_pages * page_size."""
     return int(_native.lib().fqkv_evict_workspace_bytes(B, Hkv, max_len, budget))
-
-
-def _decode_paged(op, q, K, V, Ks, Vs, block_table, seq_lens, out, workspace, weights):
-    ts = (q, K, V, block_table, seq_lens) + (() if Ks is None else (Ks, Vs))
-    idx = _gpu_of(op, *ts) if weights is None else _gpu_of(op, *ts, weights)
-    desc, B, Hkv, D, cap = _paged_kv(op, K, V, Ks, Vs, block_table, seq_lens)
-    qshape = q.shape
-    if len(qshape) != 3 or q.dtype is not _F16 or not q.is_contiguous():
-        _fail(op, "fp16", "q must be a contiguous fp16 [B, Hq, D] tensor")
-    Hq = qshape[1]
-    if qshape[0] != B or qshape[2] != D:
-        _fail(op, "shape", f"q has shape {tuple(qshape)}, expected ({B}, Hq, {D})")
-    w = None
-    if weights is not None:
-        _slot_weights(op, "weights", weights, (B, Hkv, cap))
-        w = weights.data_ptr()
-    bf16 = 0
-    if out is None:
-        out = torch.empty_like(q)
-    else:
-        _kv_out(op, q, out, qshape, q.device)
-        bf16 = 1 if out.dtype is _BF16 else 0
-    if workspace is None:
-        nb = _workspace_size(idx, "fqkv_paged_workspace_bytes", 0 if Ks is None else _native.KV_INT8, B, Hq, Hkv, D, cap,
-                             0 if w is None else 1)
-        workspace = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
-        ws = workspace.data_ptr() if nb else None
-    else:
-        ws, nb = _scratch(op, workspace, idx)
-    rc = _on_gpu(idx, _native.lib().fqkv_decode_attn_paged, desc, bf16, q.data_ptr(), out.data_ptr(), Hq, w, ws, nb,
-                 _stream_of(idx))
-    if rc:
-        _workspace_sizes.clear()
-        _native.check(rc, f"launch: {op}")
-    return out
 
 
 def decode_attn_gqa_paged(q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, block_table: torch.Tensor,
@@ -957,7 +810,8 @@ def decode_attn_gqa_paged(q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, blo
     overlap need one each) are allocated when not given.  ``weights`` [B,Hkv,max_pages*page_size] f32: each token's
     softmax weight, summed over the query heads of its KV head, is added to it (:func:`evict_kvcache_paged` reads it).
     """
-    return _decode_paged("decode_attn_gqa_paged", q, K, V, None, None, block_table, seq_lens, out, workspace, weights)
+    return _native.binding().decode("decode_attn_gqa_paged", q, K, V, None, None, block_table, seq_lens, out, workspace,
+                                    weights)
 
 
 def decode_attn_gqa_int8_paged(q, Kq, Vq, Ks, Vs, block_table, seq_lens, out=None, workspace=None,
@@ -967,7 +821,7 @@ def decode_attn_gqa_int8_paged(q, Kq, Vq, Ks, Vs, block_table, seq_lens, out=Non
     op = "decode_attn_gqa_int8_paged"
     if Ks is None or Vs is None:
         _fail(op, "fp16", "Ks and Vs are needed")
-    return _decode_paged(op, q, Kq, Vq, Ks, Vs, block_table, seq_lens, out, workspace, weights)
+    return _native.binding().decode(op, q, Kq, Vq, Ks, Vs, block_table, seq_lens, out, workspace, weights)
 
 
 def rope_axes(sections, interleaved: bool = False, device="cuda") -> torch.Tensor:
@@ -1003,49 +857,8 @@ def rope_qkv_append_paged(qkv: torch.Tensor, cos_table: torch.Tensor, sin_table:
     :func:`check_device_status`; two tokens of one call must not share a slot,
     and q_out must not overlap qkv.
     """
-    op = "rope_qkv_append_paged"
-    ts = (qkv, cos_table, sin_table, positions, slots, block_table, q_out, K, V) + _scales(op, Ks, Vs)
-    if axes is not None:
-        ts += (axes,)
-    if seq_ids is not None:
-        ts += (seq_ids,)
-    idx = _gpu_of(op, *ts)
-    desc, B, Hkv, D, _ = _paged_kv(op, K, V, Ks, Vs, block_table, None)
-    bf16 = 1 if qkv.dtype is _BF16 else 0
-    if not bf16 and qkv.dtype is not _F16:
-        _fail(op, "dtype", "qkv must be fp16 or bf16")
-    oshape, xshape = q_out.shape, qkv.shape
-    if len(oshape) != 3 or q_out.dtype is not _F16 or not q_out.is_contiguous():
-        _fail(op, "fp16", "q_out must be a contiguous fp16 [T, Hq, D] tensor")
-    T, Hq, oD = oshape
-    width = (Hq + 2 * Hkv) * D
-    if oD != D or len(xshape) != 2 or xshape[0] != T or xshape[1] < width or qkv.stride(1) != 1:
-        _fail(op, "shape", f"qkv must be [T, >= (Hq + 2 Hkv) D] with contiguous rows and q_out [T, Hq, {D}] "
-                           f"(got {tuple(xshape)}, {tuple(oshape)})")
-    tshape = cos_table.shape
-    if len(tshape) != 2 or tshape[1] != D // 2 or sin_table.shape != tshape or cos_table.dtype is not _F32 \
-            or sin_table.dtype is not _F32 or not cos_table.is_contiguous() or not sin_table.is_contiguous():
-        _fail(op, "tables", f"cos_table and sin_table must be contiguous float32 [rows, D/2 = {D // 2}]")
-    _index_vector(op, "slots", slots, T)
-    pshape = positions.shape
-    if positions.dtype is not _I32 or len(pshape) not in (1, 2) or pshape[-1] != T or (T > 1 and positions.stride(-1) != 1):
-        _fail(op, "positions", f"positions must be int32 [T = {T}] or [A, T] with contiguous rows")
-    A = pshape[0] if len(pshape) == 2 else 1
-    amap, astride = None, T
-    if A > 1:
-        if axes is None:
-            _fail(op, "axes", "several position axes need axes [D/2]")
-        _index_vector(op, "axes", axes, D // 2)
-        amap, astride = axes.data_ptr(), positions.stride(0)
-    ids = None
-    if seq_ids is not None:
-        _index_vector(op, "seq_ids", seq_ids, T)
-        ids = seq_ids.data_ptr()
-    rc = _on_gpu(idx, _native.lib().fqkv_rope_append_paged, desc, bf16, qkv.data_ptr(), qkv.stride(0) if T > 1 else width,
-                 cos_table.data_ptr(), sin_table.data_ptr(), tshape[0], positions.data_ptr(), astride, A, amap, ids,
-                 slots.data_ptr(), q_out.data_ptr(), T, Hq, _stream_of(idx))
-    if rc:
-        _native.check(rc, f"launch: {op}")
+    _native.binding().append("rope_qkv_append_paged", qkv, cos_table, sin_table, positions, slots, block_table, q_out, K, V,
+                             Ks, Vs, axes, seq_ids)
 
 
 def evict_kvcache_paged(K: torch.Tensor, V: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -1063,36 +876,8 @@ def evict_kvcache_paged(K: torch.Tensor, V: torch.Tensor, block_table: torch.Ten
     sequences must be copied first.  ``workspace``: ``evict_workspace_bytes`` bytes, allocated when not given.
     """
     op = "evict_kvcache_paged"
-    ts = (K, V, block_table, seq_lens, weights) + _scales(op, Ks, Vs)
-    if weights_out is not None:
-        ts += (weights_out,)
-    if lens_out is not None:
-        ts += (lens_out,)
-    idx = _gpu_of(op, *ts)
-    desc, B, Hkv, D, cap = _paged_kv(op, K, V, Ks, Vs, block_table, seq_lens)
-    _slot_weights(op, "weights", weights, (B, Hkv, cap))
-    if weights_out is None:
-        weights_out = weights
-    else:
-        _slot_weights(op, "weights_out", weights_out, (B, Hkv, cap))
-    if lens_out is None:
-        lens_out = torch.empty_like(seq_lens)
-    else:
-        _index_vector(op, "lens_out", lens_out, B)
     budget, recent = int(budget), int(recent)
     if not 0 <= recent <= budget:
         _fail(op, "recent", f"recent must be in [0, budget = {budget}] (got {recent})")
-    if budget > cap:  # evicts nothing; a C integer may not hold it
-        budget, recent = cap, min(recent, cap)
-    if workspace is None:
-        nb = _workspace_size(idx, "fqkv_evict_workspace_bytes", B, Hkv, cap, budget) if B else 0
-        workspace = torch.empty(nb, dtype=torch.uint8, device=K.device) if nb else None
-        ws = workspace.data_ptr() if nb else None
-    else:
-        ws, nb = _scratch(op, workspace, idx)
-    rc = _on_gpu(idx, _native.lib().fqkv_evict_paged, desc, weights.data_ptr(), weights_out.data_ptr(), lens_out.data_ptr(),
-                 budget, recent, ws, nb, _stream_of(idx))
-    if rc:
-        _workspace_sizes.clear()
-        _native.check(rc, f"launch: {op}")
-    return lens_out
+    return _native.binding().evict(op, K, V, Ks, Vs, block_table, seq_lens, weights, budget, recent, weights_out, lens_out,
+                                   workspace)
