@@ -279,7 +279,9 @@ __device__ void select_tokens(const PagedEvict& a, const float* w, int* list, in
 // `a.cluster` CTAs per (sequence, KV head), one cluster.
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_constant__ PagedEvict a) {
   __shared__ SelectShared sm;
-  pdl_launch_dependents();
+  // The move is let in only when the selection is over: where both kernels of a call let their successor in at their
+  // start, the next call's selection waits beside this one's move, and calls on end take 17.3 instead of 13.9 us (one
+  // sequence of 2112 tokens).
   pdl_wait_primary();
   const int C = a.cluster;
   const int rank = int(blockIdx.x) % C, tid = threadIdx.x;
