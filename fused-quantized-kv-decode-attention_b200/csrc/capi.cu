@@ -977,15 +977,16 @@ static int64_t paged_shape(fqkv::PagedLaunch& a, const DeviceState& ds, bool wei
   const int64_t units = int64_t(a.B) * a.Hkv * a.groups;
   const fqkv::PagedOccupancy& occ = ds.occ_paged[a.int8][a.D == 128][a.GP > 8];
   // Few units of short sequences: a cluster per unit merges its parts itself, one launch and no workspace.  The lengths are
-  // not known here, so the capacity decides, and no CTA gets more than 512 tokens: a long sequence among short ones then
-  // costs a few microseconds, where tiles in one line would be shared out evenly.  Measured (fp16, D = 128, 8 KV
-  // heads, one line -> clusters): B=1, 640 tokens 7.7 -> 5.9 us, 2048 8.4 -> 7.0, 8192 13.4 -> 13.2; B=4, 640 10.0 -> 6.6,
-  // 2048 11.4 -> 8.9; B=8, 640 11.4 -> 7.5, 2048 18.4 -> 14.6; int8 alike.  With weights the second launch stays, and one line
-  // is faster (B=1, 2048: 8.5 against 9.8 us).
+  // not known here, so the capacity decides, and no CTA gets more than 512 tokens (384 in clusters of 16): a long sequence
+  // among short ones then costs a few microseconds, where tiles in one line would be shared out evenly.  Measured (fp16,
+  // D = 128, 8 KV heads, one line -> clusters): B=1, 640 tokens 7.2 -> 5.6 us, 2048 8.5 -> 6.6, 6000 10.6 -> 10.3, 8192
+  // 11.1 -> 12.2; B=4, 640 8.3 -> 6.4, 2048 10.2 -> 8.2, 4096 14.4 -> 12.1; B=8, 640 10.3 -> 7.2, 2048 14.4 -> 12.0; int8
+  // alike (B=1, 8192: 10.9 -> 10.8).  With weights the second launch stays, and one line is faster (B=1, 2048: 8.5 against
+  // 9.8 us).
   a.cluster = 0;
   for (int k = 3; k >= 1 && !a.cluster && !weights; --k) {
     const int64_t size = int64_t(2) << k;
-    if (a.cap <= 512 * size && units <= occ.clusters[k] && size <= tiles) a.cluster = int(size);
+    if (a.cap <= (size == 16 ? 384 : 512) * size && units <= occ.clusters[k] && size <= tiles) a.cluster = int(size);
   }
   a.grid = int(a.cluster ? units * a.cluster : std::min(int64_t(ds.sm_count) * std::max(1, occ.ctas_per_sm), units * tiles));
   return tiles;
