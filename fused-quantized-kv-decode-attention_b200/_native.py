@@ -140,11 +140,15 @@ def binding():
     handle = lib()
     with _lock:
         if _binding is None:
+            import torch
+
             try:
                 from . import _torch_binding as mod
             except ImportError as exc:
-                raise NativeLibraryError(
-                    f"_torch_binding.so is not built for this torch ({exc}); run build.py in {LIB_PATH.parent}") from exc
+                raise NativeLibraryError(f"cannot load _torch_binding.so ({exc}); run build.py in {LIB_PATH.parent}") from exc
+            if mod.built_for_torch != torch.__version__:
+                raise NativeLibraryError(f"_torch_binding.so was built for torch {mod.built_for_torch}, this is "
+                                         f"{torch.__version__}; run build.py --force in {LIB_PATH.parent}")
             mod.bind(*(ctypes.cast(getattr(handle, f), ctypes.c_void_p).value
                        for f in ("fqkv_last_error", "fqkv_decode_attn_paged", "fqkv_paged_workspace_bytes",
                                  "fqkv_rope_append_paged", "fqkv_evict_paged", "fqkv_evict_workspace_bytes")))

@@ -74,7 +74,8 @@ def _build_binding(verbose: bool) -> None:
     cuda = pathlib.Path(nvcc()).resolve().parents[1] / "include"
     tmp = BINDING.with_suffix(".so.tmp")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DBUILT_FOR_TORCH="{torch.__version__}"', f"-I{INCLUDE}",
            "-isystem", sysconfig.get_paths()["include"], "-isystem", str(root / "include"),
            "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"), "-isystem", str(cuda),
            str(CSRC / "torch_binding.cpp"), "-o", str(tmp),

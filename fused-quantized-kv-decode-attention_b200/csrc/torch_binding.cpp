@@ -313,4 +313,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_binding", "The paged-cache 
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__torch_binding() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__torch_binding() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "built_for_torch", BUILT_FOR_TORCH) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

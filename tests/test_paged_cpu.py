@@ -165,6 +165,14 @@ def test_python_layer_refuses_cpu_tensors(fqkv):
         fqkv.rope_qkv_append_paged(q[0], q[0].float(), q[0].float(), i[0], i[0], i, q, K, K)
 
 
+def test_binding_of_another_torch_is_refused(fqkv, monkeypatch):
+    assert fqkv.native.binding().built_for_torch == torch.__version__
+    monkeypatch.setattr(fqkv.native, "_binding", None)
+    monkeypatch.setattr(torch, "__version__", "0.0")
+    with pytest.raises(fqkv.native.NativeLibraryError, match="built for torch"):
+        fqkv.native.binding()
+
+
 def test_rope_axes(fqkv):
     assert fqkv.rope_axes([4], device="cpu").tolist() == [0] * 4
     assert fqkv.rope_axes([2, 3, 1], device="cpu").tolist() == [0, 0, 1, 1, 1, 2]
