@@ -13,13 +13,14 @@
 // distributed-shared-memory atomics, integers, so the order does not matter.  Where the bin holds few keys (short
 // caches), each is compared with the others instead of two more digits.
 //
-// The move: bound by HBM, 2 x the kept rows (48 sequences of 16K -> 4096, D = 128, fp16: 1.65 GB in 308 us, selection
+// The move: bound by HBM, 2 x the kept rows (48 sequences of 16K -> 4096, D = 128, fp16: 1.65 GB in 305 us, selection
 // included).  In place, and the list is ascending with list[p] >= p: a row's
 // destination is at or before its source.  One CTA moves one column slice of K (or V) of one (sequence, KV
 // head), chunk by chunk in list order; a chunk is written only after it and all earlier chunks were read, and a
 // chunk's writes end below the next chunk's first source, so reading ahead is free.  Slices make enough CTAs for
 // few sequences.  The chunks before the first gap are not touched.  Two chunks of 32 KB in flight in each of three CTAs
-// per SM (three in each of two: 97 us instead of 95 us for 16 sequences; 16 KB chunks: 99 to 135 us).  (One launch,
+// per SM (three in each of two: 92 us instead of 90 us for 16 sequences, 331 us instead of 343 us for 4 of 100000 ->
+// 50000; 16 KB chunks: 99 to 135 us).  (One launch,
 // with a cluster per (sequence, KV head) that selects and then moves, was 5 us slower for one sequence -- a cluster's
 // barriers -- and no faster for many.)
 #include <cuda_fp16.h>
@@ -95,8 +96,8 @@ struct SelectShared {
 
 // One slice is read three times: for the first digit's bins, to pick out the keys in the bin chosen (the two other
 // digits then look at those alone, unless there are more than kCand of them), and for the list.
-// kMine: consecutive tokens of one thread per step (4 where a slice has no more than 4096: the selection and move of one sequence
-// of 2112 tokens take 18.4 us, with 16 tokens per thread 20.5 us).
+// kMine: consecutive tokens of one thread per step (4 where a slice has no more than 4096: the selection and move of one
+// sequence of 2112 tokens take 12.2 us, with 16 tokens per thread 15.8 us).
 template <int kMine, bool kOneStep>
 __device__ void select_tokens(const PagedEvict& a, const float* w, int* list, int rank, int s0, int s1, int k,
                               SelectShared& sm) {
@@ -571,17 +572,19 @@ cudaError_t launch_evict_paged(const PagedEvict& args, cudaStream_t stream) {
   PagedEvict a = args;
   const int units = a.kv.B * a.kv.Hkv;
   // The move: column slices until about 600 CTAs exist, none narrower than 64 bytes (a DRAM access: 4 sequences of
-  // 100000 -> 50000, 8 KV heads, D = 128: 4 slices of 64 bytes 357 us, 8 of 32 bytes 482 us); 32 bytes only where there
-  // would not be a CTA per SM (one sequence of 16K -> 4096: 34 us in 64, 28 us in 128 CTAs).  16 sequences of 0 to
-  // 16K -> 4096: 2 slices 95 us, 4 slices 90 us; 48 of 12K to 16K: 1 slice 308 us, 2 slices 322 us.
+  // 100000 -> 50000, 8 KV heads, D = 128: 4 slices of 64 bytes 343 us, 8 of 32 bytes 438 us); 32 bytes only where there
+  // would not be a CTA per SM (one sequence of 16K -> 4096: 24 us in 64, 22 us in 128 CTAs).  16 sequences of 0 to
+  // 16K -> 4096: 2 slices 93 us, 4 slices 90 us; 48 of 12K to 16K: 1 slice 305 us, 2 slices 315 us.
   a.slices = 1;
   const auto width = [&] { return a.kv.D * (a.kv.int8 ? 1 : 2) / a.slices; };
   while ((units * 2 * a.slices < 600 && width() > 64) || (units * 2 * a.slices < a.sms && width() > 32)) a.slices *= 2;
   // The selection: one CTA while a full sequence is about what it holds in registers (one step and a half, so that a
-  // table with room to spare for 16K tokens does not pay a cluster's barriers: 31 us instead of 35 us for one such
-  // sequence of 8 KV heads), then clusters of 2, 4 and 8.
+  // table with room to spare for 16K tokens does not pay a cluster's barriers: 22.1 us instead of 25.6 us for one such
+  // sequence of 8 KV heads), then clusters of 2, 4 and 8, as long as every CTA has an SM to itself: 1 sequence of 48K ->
+  // 12K 42 us in clusters of 2 and 57 us without, 16 of them 347 us and 322 us, 16 of 100K 737 us in 8 and 667 us without.
   a.cluster = 1;
-  while (a.cluster < 8 && int64_t(a.cluster) * (kMost + kMost / 2) < a.kv.cap) a.cluster *= 2;
+  while (a.cluster < 8 && units * a.cluster * 2 <= a.sms && int64_t(a.cluster) * (kMost + kMost / 2) < a.kv.cap)
+    a.cluster *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(units) * unsigned(a.cluster));
   cfg.blockDim = dim3(kSelThreads);

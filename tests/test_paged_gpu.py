@@ -672,6 +672,16 @@ def test_evict_long(fqkv, n, budget, recent):
     _clean(fqkv)
 
 
+@pytest.mark.parametrize("lens,Hkv,budget,recent", [([100001, 77], 1, 700, 30), ([26001, 40, 31000, 0] + [301] * 20, 4, 300, 11),
+                                                    ([26001] + [9] * 8, 4, 6000, 0)])
+def test_evict_long_by_clusters_and_by_one_block(fqkv, lens, Hkv, budget, recent):
+    """Eight blocks per selection; one block in several steps, where there are many (sequence, head) pairs."""
+    c = Cache(fqkv, lens, Hkv, 64, 64, False, seed=budget)
+    w = torch.randn(c.B, Hkv, c.cap, generator=torch.Generator().manual_seed(budget)).exp().mul(8).floor().cuda()
+    _evict_check(fqkv, c, w, budget, recent)
+    _clean(fqkv)
+
+
 def test_evict_odd_weights(fqkv):
     """NaN above +inf above numbers, both zeros alike, negative weights, all equal."""
     c = Cache(fqkv, [200, 200, 200, 200], 1, 64, 16, False)
