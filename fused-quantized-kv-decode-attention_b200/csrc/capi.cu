@@ -981,10 +981,12 @@ static int64_t paged_shape(fqkv::PagedLaunch& a, const DeviceState& ds, bool wei
   // among short ones then costs a few microseconds, where tiles in one line would be shared out evenly.  Measured (fp16,
   // D = 128, 8 KV heads, one line -> clusters): B=1, 640 tokens 7.2 -> 5.6 us, 2048 8.5 -> 6.6, 6000 10.6 -> 10.3, 8192
   // 11.1 -> 12.2; B=4, 640 8.3 -> 6.4, 2048 10.2 -> 8.2, 4096 14.4 -> 12.1; B=8, 640 10.3 -> 7.2, 2048 14.4 -> 12.0; int8
-  // alike (B=1, 8192: 10.9 -> 10.8).  With weights the second launch stays, and one line is faster (B=1, 2048: 8.5 against
-  // 9.8 us).
+  // alike (B=1, 8192: 10.9 -> 10.8); in pairs of CTAs B=16, 640 11.5 -> 9.0, 1024 14.8 -> 12.0.  Lengths from 0 to the
+  // capacity: B=16, 640 11.0 -> 8.7, 1024 11.6 -> 11.6, B=8, 2048 11.0 -> 11.5; one of 2048 among seven of 40: 9.2 -> 10.9.
+  // (A CTA per unit: -2 to +2 us, not taken.)  With weights the second launch stays, and one line is faster (B=1, 2048: 8.5
+  // against 9.8 us).
   a.cluster = 0;
-  for (int k = 3; k >= 1 && !a.cluster && !weights; --k) {
+  for (int k = 3; k >= 0 && !a.cluster && !weights; --k) {
     const int64_t size = int64_t(2) << k;
     if (a.cap <= (size == 16 ? 384 : 512) * size && units <= occ.clusters[k] && size <= tiles) a.cluster = int(size);
   }

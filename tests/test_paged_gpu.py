@@ -408,9 +408,9 @@ def test_attention_graph_follows_lengths_and_shares_a_workspace(fqkv, int8):
 
 @pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("lens,Hkv", [([8000], 1), ([3900, 10], 8), ([2000, 1, 0, 700, 2040, 5, 64, 1999], 8), ([120] * 9, 3),
-                                      ([6000], 1), ([3900, 10, 2500, 64], 8), ([1000] * 9, 8)])
+                                      ([6000], 1), ([3900, 10, 2500, 64], 8), ([1000] * 9, 8), ([1000] * 14 + [0, 1, 513, 512], 8)])
 def test_attention_clusters_of_every_size(fqkv, int8, lens, Hkv):
-    """Sixteen, eight and four CTAs per unit, with CTAs that get no tile."""
+    """Sixteen, eight, four and two CTAs per unit, with CTAs that get no tile."""
     c = Cache(fqkv, lens, Hkv, 128, 64, int8, seed=len(lens), extra_pages=0)
     q = _q(c.B, Hkv * 3, 128, sigma=2.0)
     out = c.attend(fqkv, q)
