@@ -36,7 +36,11 @@
 //    rounded to fp16, times a power of two that puts the unit's largest V scale so far in [2^13, 2^14): small
 //    scales keep all their bits, and the factor leaves exactly at the end of the unit.
 //  * Scores, maxima, sums and outputs are fp32; the probabilities are rounded to fp16 once, as the operand of
-//    the second product (half an ulp is 2^-12 relative, random over the keys); the output is rounded once.
+//    the second product; the output is rounded once.  fp16 cache: times 2^15 first (1 becomes 32768, below fp16's
+//    largest), and O times 2^-15 at the end of a unit, both exact.  So a probability down to 2^-29 of the warp's
+//    largest has all its 11 bits (half a step is at most 2^-11 relative), and one below is off by 2^-40 of the
+//    largest at most: beside a dominant key the many small ones of a long cache keep their sum (unscaled, half a
+//    step is 2^-25: equal weights of 2^-24.5 came out 1.41 times too large, of 2^-25.1 as nothing).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -247,6 +251,7 @@ __device__ __forceinline__ uint32_t codes_to_half2(uint32_t x) {
   return h;
 }
 constexpr uint32_t kMinus1152 = 0xE480E480u;  // two fp16 -1152
+constexpr float kProbScale = 32768.f;         // of an fp16 cache's probabilities as MMA operands
 
 // D(16x8, s32) += A(16x32, s8, row) * B(32x8, s8, col).
 __device__ __forceinline__ void mma_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -654,7 +659,8 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const float* s2 = &sc[2 * kb + i][2 * nt];
-              pb[nt][i] = kI8 ? pack_half2(s2[0] * vs[2 * kb + i][0], s2[1] * vs[2 * kb + i][1]) : pack_half2(s2[0], s2[1]);
+              pb[nt][i] = kI8 ? pack_half2(s2[0] * vs[2 * kb + i][0], s2[1] * vs[2 * kb + i][1])
+                              : pack_half2(s2[0] * kProbScale, s2[1] * kProbScale);
             }
           const uint32_t at = sv + v_off + uint32_t(16 * kb * C::RB);
           if constexpr (!kI8) {
@@ -710,7 +716,7 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
     // ---- end of the part: merge the warps; write the output (a whole unit) or one part of it
     const bool whole = p.t0 == 0 && p.t1 == p.nt;
     const size_t slot = size_t(blockIdx.x) * 2 + (p.t0 == 0 ? 1 : 0);
-    const float unframe = (kI8 && frame != 0.f) ? 1.f / frame : 1.f;
+    const float unframe = !kI8 ? 1.f / kProbScale : frame != 0.f ? 1.f / frame : 1.f;
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
       float l = l_run[nt];
