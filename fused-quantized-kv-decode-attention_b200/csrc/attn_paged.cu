@@ -33,8 +33,8 @@
 //    a constant tile takes 1152 P away again, 16 keys at a time: the subtraction costs tensor-core time, which is
 //    there, and no instruction per code; what it rounds is 2^-24 of 1152 P, 7e-5 of a code's step.  The K scale multiplies
 //    the score.  The V scale multiplies the probability before it is
-//    rounded to fp16, times a power of two that puts the unit's largest V scale so far in [2^13, 2^14): small
-//    scales keep all their bits, and the factor leaves exactly at the end of the unit.
+//    rounded to fp16, times a power of two that puts the unit's largest V scale so far (by magnitude) in
+//    [2^13, 2^14): small scales keep all their bits, and the factor leaves exactly at the end of the unit.
 //  * Scores, maxima, sums and outputs are fp32; the probabilities are rounded to fp16 once, as the operand of
 //    the second product; the output is rounded once.  fp16 cache: times 2^15 first (1 becomes 32768, below fp16's
 //    largest), and O times 2^-15 at the end of a unit, both exact.  So a probability down to 2^-29 of the warp's
@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
         if constexpr (kI8) {
           float vmax = 0.f;
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) vmax = fmaxf(vmax, fmaxf(vs[j][0], vs[j][1]));
+          for (int j = 0; j < NJ; ++j) vmax = fmaxf(vmax, fmaxf(fabsf(vs[j][0]), fabsf(vs[j][1])));  // either sign
           vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 1));
           vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));  // the same in every lane
           if (vmax * frame >= 16384.f || (frame == 0.f && vmax > 0.f)) {

@@ -80,3 +80,27 @@ def test_long_sequences_with_a_dominant_key(fqkv, int8):
     out = c.attend(fqkv, q.expand(B, -1, -1).contiguous()).double().cpu().numpy()
     assert (np.abs(out - r["out"]) <= _bound(r, n, D, int8)).all(), np.abs(out / r["out"] - 1).max((0, 2))
     _clean(fqkv)
+
+
+@pytest.mark.parametrize("D,Hq", [(64, 4), (128, 8), (128, 24)])
+@PLANS
+def test_int8_scales_of_either_sign(fqkv, D, Hq, line):
+    """V scales all negative, of both signs, and negative first; K scales of both signs."""
+    c = Cache(fqkv, [300, 300, 300], 2, D, 16, True, seed=D)
+    g = torch.Generator().manual_seed(4)
+    sign = (torch.randint(2, c.Ks.shape, generator=g) * 2 - 1).half().cuda()
+    c.Ks = c.Ks * sign
+    c.Vs[c.table[0, :19].long()] *= -1
+    c.Vs = c.Vs.contiguous()
+    for i in range(19):
+        c.Vs[int(c.table[1, i])] *= sign[int(c.table[1, i])]
+        if i < 9:  # small negative ones, then larger positive ones
+            c.Vs[int(c.table[2, i])] *= -2.0 ** -6
+    if line:
+        c.widen()
+    q = _q(3, Hq, D)
+    c.check(fqkv, q, c.attend(fqkv, q))
+    w = torch.zeros(3, 2, c.cap, device="cuda")
+    out = c.attend(fqkv, q, weights=w)
+    c.check(fqkv, q, out, torch.zeros_like(w), w)
+    _clean(fqkv)
