@@ -317,13 +317,13 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
 
   // ------------------------------------------------------------ producer
   if (warp == kWarps) {
-    if (!a.debug_skip_loads) {
+    int it = 0;
+    if (a.debug_skip_loads != 1) {
       const int br = a.box;             // keys per box
       const int nb = C::TK / br;        // boxes per tile: 1, 2, 4 or 8
       constexpr int kKinds = 2 * C::kBlocks;  // copies per box
       const int job_box = lane / kKinds, kind = lane % kKinds;
       const int sc_key = (lane % (C::TK / 8)) * 8;  // int8: 8 scales of K (the lower lanes) or of V
-      int it = 0;
       bool ok = true;
       while (ok && walk.next(p)) {
         const int* row = a.table + int64_t(p.b) * a.table_stride;
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
           __syncwarp();
           uint8_t* stage = smem + size_t(st) * C::kStageBytes;
           const int id = __shfl_sync(0xffffffffu, ids, (at + job_box) & 31);
-          if (job_box < boxes) {
+          if (job_box < boxes && !a.debug_skip_loads) {
             const int tok = a.page_div.mod(t * C::TK + job_box * br);
             const bool known = unsigned(id) < unsigned(a.num_pages);
             if (!known && kind == 0) atomicCAS(a.status, kDevOk, kDevBadPage);
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
             // bounds small pages (D = 64, 16-token pages, B = 64, 4K: 77 us with, 72 us without)
             const int sc_box = sc_key / br;
             const int sid = __shfl_sync(0xffffffffu, ids, (at + sc_box) & 31);
-            if (sc_box < boxes) {
+            if (sc_box < boxes && !a.debug_skip_loads) {
               const int pg = unsigned(sid) < unsigned(a.num_pages) ? sid : 0;  // some scales for zero codes
               const int tok = a.page_div.mod(t * C::TK + sc_key);
               const __half* src = lane < C::TK / 8 ? a.Ks + pg * a.ks_page + p.kh * a.ks_head + tok
@@ -377,17 +377,17 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
           }
         }
       }
-      if (!ok && lane == 0) {
-        // The consumers gave up: wait (bounded) for the copies in flight before the CTA's memory goes.
-        for (int j = (it > C::kStages ? it - C::kStages : 0); j < it; ++j)
-          mbar_wait(&full[j % C::kStages], (j / C::kStages) & 1, wc, kDevTimeoutDrain);
-      }
     }
     // The stream's next kernel is let in by a cluster when its last copy is under way, by the line's CTAs only when they
     // leave.  Calls on end (letting it in at the start / here / not at all): cluster, 5 odd int8 sequences 10.1 / 9.5 /
     // 9.5 us, one of 640 tokens 4.9 / 4.8 / 5.2 us (in a graph); line, 6 sequences of 0 to 5000 tokens 16.0 / 15.3 /
     // 14.4 us, 16 of 0 to 8K 51.6 / 50.6 / 49.9 us.
     if constexpr (kCl) pdl_launch_dependents();
+    // The copies in flight land (a bounded wait) before the CTA's memory goes: consumers that gave up do not wait for them,
+    // and the loop above does not notice that when they did so behind its last free stage.
+    if (lane == 0)
+      for (int j = max(0, it - C::kStages); j < it; ++j)
+        mbar_wait(&full[j % C::kStages], (j / C::kStages) & 1, wc, kDevTimeoutDrain);
     if constexpr (kCl) {  // the whole warp takes part in the consumers' two cluster barriers
       __syncwarp();
       cluster_sync_all();
@@ -407,7 +407,8 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
   const uint32_t v_off = blk_off<C::RB>(r0 + ((mi & 1) << 3) + rr, mi >> 1);
   const uint32_t ring = smem_u32(smem);
   const int ct = threadIdx.x;
-  bool alive = true;
+  bool alive = a.debug_skip_loads != 2;
+  if (!alive && lane == 0) abort_flag = 1;
   int it = 0;
 
   // a cluster's CTA leaves its part here, in the ring, when all its tiles have been used
@@ -769,10 +770,12 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
           for (int i = 0; i < kDims; ++i) O[i] += wt[w] * v[i];
         }
         if constexpr (kCl) {
-          if (lane == 0) *reinterpret_cast<float2*>(cl_ml + 2 * hh) = make_float2(M, L);
-          float* dst = cl_o + hh * D + lane * kDims;
-          if constexpr (kDims == 4) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(O);
-          else *reinterpret_cast<float2*>(dst) = *reinterpret_cast<const float2*>(O);
+          if (alive) {  // this warp has seen every tile arrive, so no copy is on its way into the ring
+            if (lane == 0) *reinterpret_cast<float2*>(cl_ml + 2 * hh) = make_float2(M, L);
+            float* dst = cl_o + hh * D + lane * kDims;
+            if constexpr (kDims == 4) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(O);
+            else *reinterpret_cast<float2*>(dst) = *reinterpret_cast<const float2*>(O);
+          }
         } else if (whole) {
           const float r = 1.f / L;
 #pragma unroll

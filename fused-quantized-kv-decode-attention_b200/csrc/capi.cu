@@ -511,7 +511,7 @@ const char* fqkv_version(void) { return "fqkv_b200 0.1.0 (sm_100a)"; }
 
 void fqkv_set_wait_timeout_ms(uint32_t ms) { g_timeout_ns.store(uint64_t(ms) * 1000000ull); }
 
-void fqkv_debug_skip_loads(int enable) { g_debug_skip_loads.store(enable ? 1 : 0); }
+void fqkv_debug_skip_loads(int enable) { g_debug_skip_loads.store(enable == 2 ? 2 : enable ? 1 : 0); }
 
 int fqkv_set_split_mode(int mode) {
   if (mode != FQKV_SPLIT_AUTO && mode != FQKV_SPLIT_COMBINE && mode != FQKV_SPLIT_CLUSTER)

@@ -235,7 +235,7 @@ struct PagedLaunch {
   float sm_scale_log2;
   int* status;
   unsigned long long timeout_ns;
-  int debug_skip_loads;
+  int debug_skip_loads;    // test hook: 1 nothing is issued; 2 tiles are announced, not issued, and nobody waits for them
   bool int8, out_bf16;
 };
 int paged_tile_keys(bool int8);
