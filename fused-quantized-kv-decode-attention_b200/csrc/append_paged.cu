@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kAppendThreads + 32) append_many_kernel(const 
 
   // ------------------------------------------------------------ producer
   if (warp == kAppendThreads / 32) {
-    if (a.debug_skip_loads) return;
+    if (a.debug_skip_loads == 1) return;
     constexpr int kPairs = D / 64;  // rotary pairs per lane
     int axis[kPairs];
 #pragma unroll
@@ -265,16 +265,12 @@ __global__ void __launch_bounds__(kAppendThreads + 32) append_many_kernel(const 
     place();
     look(int64_t(blockIdx.x) + gridDim.x);
     int it = 0;
-    bool ok = true;
     for (int64_t token = blockIdx.x; token < a.T; token += gridDim.x, ++it) {
       const int st = it % kRowStages;
       if (it >= kRowStages) {
         const bool free_stage = !*reinterpret_cast<volatile int*>(&abort_flag) &&
                                 mbar_wait(&empty[st], ((it / kRowStages) - 1) & 1, wc, kDevTimeoutEmpty);
-        if (!__all_sync(0xffffffffu, free_stage)) {
-          ok = false;
-          break;
-        }
+        if (!__all_sync(0xffffffffu, free_stage)) break;
       }
       bool good = placed1;
 #pragma unroll
@@ -283,15 +279,15 @@ __global__ void __launch_bounds__(kAppendThreads + 32) append_many_kernel(const 
       const bool known = unsigned(page1) < unsigned(a.kv.num_pages);
       uint8_t* stage = ring + size_t(st) * stage_bytes;
       float* table = reinterpret_cast<float*>(stage + row_bytes);
-      const bool put = slot1 >= 0 && good && known;
+      const bool put = slot1 >= 0 && good && known, send = put && !a.debug_skip_loads;
       if (lane == 0) {
         // padding is passed over; a wrong place or angle is recorded
         if (slot1 >= 0 && !put) atomicCAS(a.status, kDevOk, good ? kDevBadPage : kDevBadToken);
         *reinterpret_cast<RowStage*>(stage + row_bytes + D * 4) = RowStage{put ? slot1 : -1, page1};
         mbar_arrive_expect_tx(&full[st], put ? row_bytes : 0u);
-        if (put) bulk_g2s(stage, static_cast<const uint16_t*>(a.qkv) + token * a.qkv_stride, row_bytes, &full[st]);
+        if (send) bulk_g2s(stage, static_cast<const uint16_t*>(a.qkv) + token * a.qkv_stride, row_bytes, &full[st]);
       }
-      if (put) {
+      if (send) {
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
           const int64_t at = int64_t(pos1[i]) * (D / 2) + lane + 32 * i;
@@ -303,10 +299,11 @@ __global__ void __launch_bounds__(kAppendThreads + 32) append_many_kernel(const 
       place();
       look(token + 2 * int64_t(gridDim.x));
     }
-    if (!ok && lane == 0) {
-      for (int i = (it > kRowStages ? it - kRowStages : 0); i < it; ++i)
+    // The copies in flight land (a bounded wait) before the block's memory goes, whether the consumers are there for them
+    // or gave up.
+    if (lane == 0)
+      for (int i = max(0, it - kRowStages); i < it; ++i)
         mbar_wait(&full[i % kRowStages], (i / kRowStages) & 1, wc, kDevTimeoutDrain);
-    }
     return;
   }
 
@@ -315,7 +312,7 @@ __global__ void __launch_bounds__(kAppendThreads + 32) append_many_kernel(const 
   int it = 0;
   for (int64_t token = blockIdx.x; token < a.T; token += gridDim.x, ++it) {
     const int st = it % kRowStages;
-    const bool ok = mbar_wait(&full[st], (it / kRowStages) & 1, wc, kDevTimeoutFull) &&
+    const bool ok = a.debug_skip_loads != 2 && mbar_wait(&full[st], (it / kRowStages) & 1, wc, kDevTimeoutFull) &&
                     !*reinterpret_cast<volatile int*>(&abort_flag);
     if (!__all_sync(0xffffffffu, ok)) {
       if (lane == 0) abort_flag = 1;

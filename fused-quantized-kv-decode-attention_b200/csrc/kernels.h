@@ -266,7 +266,7 @@ struct PagedAppend {
   int sms;
   int* status;
   unsigned long long timeout_ns;
-  int debug_skip_loads;
+  int debug_skip_loads;    // as in PagedLaunch
 };
 cudaError_t append_paged_prepare();
 cudaError_t launch_append_paged(const PagedAppend& a, bool bf16, cudaStream_t stream);

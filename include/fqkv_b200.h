@@ -73,8 +73,8 @@ void fqkv_set_wait_timeout_ms(uint32_t ms);
  * staged quantizers (D = 64, 128, 256) issue no tile loads, so every in-kernel
  * wait for a tile runs out after the wait limit; the kernel then unwinds (no
  * load is in flight), records status 61 in the device status word and
- * returns, leaving the context usable.  2, in the paged attention:
- * tiles are announced to their barriers but not
+ * returns, leaving the context usable.  2, in the paged attention and the
+ * paged append of prompts: tiles are announced to their barriers but not
  * issued, and the consumers give up at once, so that what is left to run out
  * is the producers' wait for copies in flight (status 63).  Outputs of such
  * launches are undefined.  Never enable it outside tests. */

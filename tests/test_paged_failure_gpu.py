@@ -4,7 +4,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_paged_gpu import PLANS, Cache, _clean, _q
+from test_paged_gpu import PLANS, Cache, _clean, _q, _tables
 
 pytestmark = pytest.mark.gpu
 
@@ -35,4 +35,23 @@ def test_attention_waits_for_copies_in_flight(fqkv, int8, line):
     q = _q(2, 8, 128)
     assert _announced_only(fqkv, lambda: c.attend(fqkv, q)) == 63
     c.check(fqkv, q, c.attend(fqkv, q))
+    _clean(fqkv)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_append_waits_for_copies_in_flight(fqkv, int8):
+    """As above: 1200 tokens, one or two for a block."""
+    D, Hq, Hkv, T = 64, 4, 2, 1200
+    c = Cache(fqkv, [0, 0], Hkv, D, 16, int8, room=600)
+    cos, sin = _tables(600, D)
+    i = torch.arange(T, dtype=torch.int32).cuda()
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * D, generator=torch.Generator().manual_seed(1)).half().cuda()
+    q_out = torch.zeros(T, Hq, D, dtype=torch.float16, device="cuda")
+    call = lambda: fqkv.rope_qkv_append_paged(qkv, cos, sin, i % 600, i % 600, c.table, q_out, c.K, c.V, c.Ks, c.Vs,  # noqa: E731
+                                              seq_ids=i // 600)
+    assert _announced_only(fqkv, call) == 63
+    assert not bool(q_out.any())
+    call()
+    torch.cuda.synchronize()
+    assert bool((q_out != 0).flatten(1).any(1).all())
     _clean(fqkv)
