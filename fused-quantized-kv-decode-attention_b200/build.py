@@ -7,8 +7,10 @@ linked into ``libfqkv_b200.so`` next to this file with the CUDA runtime linked
 statically, so the library depends only on the NVIDIA driver.  ``-Xptxas -v``
 register / spill / shared-memory reports are written to
 ``_build/ptxas_<name>.log``.  ``csrc/torch_binding.cpp`` becomes the extension
-module ``_torch_binding.so`` (g++, the installed torch's headers).  Rebuilds
-only when a source or header is newer than the libraries (or with ``--force``).
+module ``_torch_binding.so`` (g++, the installed torch's headers); without
+torch it is left out, and the library alone is built for users of the C entry
+points.  Rebuilds only what a source or header is newer than (or all, with
+``--force``).
 """
 from __future__ import annotations
 
@@ -46,12 +48,11 @@ def sources() -> list[pathlib.Path]:
     return sorted(CSRC.glob("*.cu"))
 
 
-def _stale() -> bool:
-    if not LIB.exists() or not BINDING.exists():
+def _stale(target: pathlib.Path, deps: list[pathlib.Path]) -> bool:
+    if not target.exists():
         return True
-    t = min(LIB.stat().st_mtime, BINDING.stat().st_mtime)
-    deps = list(CSRC.glob("*")) + list(INCLUDE.glob("*.h")) + [pathlib.Path(__file__)]
-    return any(p.stat().st_mtime > t for p in deps)
+    t = target.stat().st_mtime
+    return any(p.stat().st_mtime > t for p in [*deps, *INCLUDE.glob("*.h"), pathlib.Path(__file__)])
 
 
 def _compile(src: pathlib.Path, verbose: bool) -> pathlib.Path:
@@ -67,8 +68,12 @@ def _compile(src: pathlib.Path, verbose: bool) -> pathlib.Path:
 
 
 def _build_binding(verbose: bool) -> None:
-    """The Python layer of the paged-cache operators, against the torch of this interpreter."""
-    import torch
+    """The Python layer of the paged-cache operators, against the torch of this interpreter (if there is one)."""
+    try:
+        import torch
+    except ImportError as exc:
+        print(f"not built: {BINDING.name}, the Python calls of the paged cache ({exc})", file=sys.stderr)
+        return
 
     root = pathlib.Path(torch.__file__).resolve().parent
     cuda = pathlib.Path(nvcc()).resolve().parents[1] / "include"
@@ -88,15 +93,8 @@ def _build_binding(verbose: bool) -> None:
         print(f"built {BINDING}")
 
 
-def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
-    if not force and not _stale():
-        return LIB
-    BUILD.mkdir(exist_ok=True)
-    srcs = sources()
-    with cf.ThreadPoolExecutor(max_workers=min(len(srcs) + 1, os.cpu_count() or 4)) as ex:
-        binding = ex.submit(_build_binding, verbose)
-        objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
-        binding.result()
+def _build_lib(ex: cf.Executor, verbose: bool) -> None:
+    objs = list(ex.map(lambda s: _compile(s, verbose), sources()))
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", str(tmp), *map(str, objs)]
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -105,6 +103,18 @@ def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
     os.replace(tmp, LIB)
     if verbose:
         print(f"built {LIB}")
+
+
+def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
+    lib = force or _stale(LIB, [*sources(), *CSRC.glob("*.h"), *CSRC.glob("*.cuh")])
+    binding = force or _stale(BINDING, [CSRC / "torch_binding.cpp"])
+    BUILD.mkdir(exist_ok=True)
+    with cf.ThreadPoolExecutor(max_workers=min(len(sources()) + 1, os.cpu_count() or 4)) as ex:
+        other = ex.submit(_build_binding, verbose) if binding else None
+        if lib:
+            _build_lib(ex, verbose)
+        if other:
+            other.result()  # its errors come behind a library that is whole
     return LIB
 
 
