@@ -825,10 +825,12 @@ def decode_attn_gqa_int8_paged(q, Kq, Vq, Ks, Vs, block_table, seq_lens, out=Non
 
 
 def rope_axes(sections, interleaved: bool = False, device="cuda") -> torch.Tensor:
-    """The position axis of each rotary pair, int32 [sum(sections)]: ``sections[a]`` pairs turn with axis a.
+    """The position axis of each of the sum(sections) rotary pairs, int32.
 
-    Contiguous: axis 0's pairs first, then axis 1's, and so on.  Interleaved: pair i < A * sections[i % A] belongs
-    to axis i % A (A axes), the others to axis 0, so every axis gets high and low frequencies.
+    Contiguous: axis 0's ``sections[0]`` pairs first, then axis 1's, and so on.  Interleaved (A axes): pair i belongs to
+    axis i % A if i < A * sections[i % A], else to axis 0, so every axis gets high and low frequencies.  Axis a > 0 then
+    has ``sections[a]`` pairs, but never more than there are pairs i with i % A == a; what it asks for beyond them stays
+    with axis 0 ([16, 24, 24] gives 22, 21 and 21 pairs; [24, 20, 20] gives just these).
     """
     sections = [int(s) for s in sections]
     if not sections or min(sections) < 0:
