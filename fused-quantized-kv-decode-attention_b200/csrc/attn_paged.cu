@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
             sc[j][2 * nt] = (!kMask || k0 + kq < p.len) ? sc[j][2 * nt] * (kI8 ? qs * kf.x : qs) : -INFINITY;
             sc[j][2 * nt + 1] = (!kMask || k0 + kq + 1 < p.len) ? sc[j][2 * nt + 1] * (kI8 ? qs * kf.y : qs) : -INFINITY;
           }
-          if (a.scores) {
+          if (!kCl && a.scores) {  // (with weights the work is never split by clusters)
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt)
               if (g + 8 * nt < gvalid && (!kMask || k0 + kq < p.len))  // cap is even: the pair stays in the row
@@ -832,7 +832,6 @@ __global__ void __launch_bounds__(kThr, (Cfg<D, kI8>::kCtas)) paged_attn_kernel(
       }
       const bool none = walk.len == 0;  // an empty sequence: zeros
       store_out2(a, (row_base + hh) * D + d, none ? 0.f : O.x / L, none ? 0.f : O.y / L);
-      if (d == 0 && a.scores) a.row_ml[row_base + hh] = make_float2(M, L);
     }
     cluster_sync_all();  // nobody leaves while its part is read
   }
