@@ -784,7 +784,8 @@ def quant_int4_per_token(X: torch.Tensor):
 # ------------------------------------------------------------------ paged KV cache
 # A decode step calls these every layer: their checks and launches are compiled (csrc/torch_binding.cpp).
 def paged_workspace_bytes(kv_format: str, B: int, Hq: int, Hkv: int, max_len: int, D: int, weights: bool = False) -> int:
-    """Workspace of a paged decode call on the current device; max_len = max_pages * page_size."""
+    """Workspace of a paged decode call on the current device; max_len = max_pages * page_size.  With ``weights``:
+    4 * B * Hq * max_len bytes of scores beside the rest, whatever the lengths are."""
     fmt = {"fp16": _native.KV_F16, "int8": _native.KV_INT8}[kv_format]
     return int(_native.lib().fqkv_paged_workspace_bytes(fmt, B, Hq, Hkv, D, max_len, 1 if weights else 0))
 

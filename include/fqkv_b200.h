@@ -379,7 +379,9 @@ typedef struct fqkv_paged_kv {
  * past the length are left as they are.  Workspace:
  * fqkv_paged_workspace_bytes(kv_format, B, Hq, Hkv, D, max_pages * page_size,
  * weights != NULL), scratch only: nothing is kept between calls, and calls
- * that may overlap need one each. */
+ * that may overlap need one each.  With weights it holds every head's scores:
+ * 4 * B * Hq * max_pages * page_size bytes beside the rest, by the table's
+ * width whatever the lengths are. */
 int fqkv_decode_attn_paged(const fqkv_paged_kv_t* kv, int32_t out_dtype, const void* q, void* o, int64_t Hq,
                            float* weights, void* workspace, size_t workspace_bytes, fqkv_stream_t stream);
 size_t fqkv_paged_workspace_bytes(int kv_format, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len,
